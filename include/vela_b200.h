@@ -175,6 +175,78 @@ int vela_fused_attention_stalled(void* stream, const int8_t* qhi, const int8_t* 
                                  int32_t* out, uint32_t* rowmax, long long wait_limit_cycles);
 
 /* ---------------------------------------------------------------------------------
+ * 4-bit decoding operators of a language model (no reference counterpart): the residual + RMS norm that writes
+ * 8-bit rows, products of a few rows with 4-bit weights, and a mixture-of-experts layer on such weights.
+ * Activations are 16- or 32-bit floats or 8-bit values with scales, row-major, `ld*` in elements.  Sums, norms and
+ * softmax statistics are held in 32 bits.  None of the calls allocates or synchronises; each may be captured in a
+ * CUDA graph.  Results do not depend on the stream, the run or what else runs (no floating-point atomics).
+ * ------------------------------------------------------------------------------ */
+#define VELA_T_BF16 0
+#define VELA_T_F16  1
+#define VELA_T_F32  2
+#define VELA_T_I8   3     /* int8 with float scales */
+#define VELA_T_E4M3 4     /* 8-bit float (4 exponent, 3 mantissa bits, largest 448) with float scales */
+
+/* h = X + R;  S = h;  y = h / sqrt(mean(h^2) + eps) * g;  Y = y;  Q * qscale ~ y.
+ * X, R, g, S, Y have the type `type` (bf16, f16, f32); R may be NULL (h = X); S, Y and Q may be NULL (not written).
+ * The mean and y use h before S's rounding.  S may be X or R itself (with the same ld); other overlaps are not allowed.
+ * Q [M, C] int8 or e4m3 (`qtype`) with qscale [M][ceil(C / qgroup)] (qgroup 64 or 128: one scale for each group of
+ * columns) or [M] (qgroup 0: one for each row): qscale = max(max|y|, 1e-30) / 127 or / 448, Q = y / qscale rounded to
+ * nearest even and kept within +-127 / +-448.  A NaN in a row makes all of its scales NaN, an infinity that of its own group
+ * (or row). */
+int vela_rms_norm_q8(void* stream, int type, const void* X, int ldx, const void* R, int ldr, const void* g, float eps, int M, int C,
+                     void* S, int lds, void* Y, int ldy, int qtype, void* Q, int ldq, float* qscale, int qgroup);
+
+/* 4-bit weights [N, K] in the library's layout.  Value (n, k) = (code - zero) * scale; codes 0..15, one scale (bf16 or
+ * f16) and zero point (0..15; 8 where `zero` is NULL) for each row and group of `group` columns (32, 64 or 128).
+ * q: tiles of 16 rows x 64 columns, 512 bytes each, row tiles outermost, N padded to 16 and K to 64 (padding is read but
+ * never used).  Byte 16 (4 g + t) + 8 h + 4 j + b of a tile (g < 8, t < 4, h < 2, j < 2, b < 4) holds column
+ * 32 h + 8 t + 4 j + {0, 2, 1, 3}[b] of row g in its low and of row g + 8 in its high four bits.
+ * scale, zero: [row tile][group][row % 8][row / 8 % 2].  q and scale are 16-byte aligned, zero 2-byte. */
+typedef struct vela_w4 {
+    const uint8_t* q; const void* scale; const uint8_t* zero;
+    int N, K, group, scale_type;      /* scale_type: VELA_T_BF16 or VELA_T_F16 */
+} vela_w4;
+/* bytes of q, and elements of scale (and of zero), for one matrix; 0 for sizes that are not allowed */
+size_t vela_w4_bytes(int N, int K);
+size_t vela_w4_scales(int N, int K, int group);
+/* host: codes [N][K] (one per byte), scales [N][ceil(K / group)] and zeros (same shape, or NULL) into the layout above;
+ * scales are rounded to scale_type, padding is written as zero.  zero is NULL exactly where zeros is. */
+int vela_w4_pack(const uint8_t* codes, const float* scales, const uint8_t* zeros, int N, int K, int group, int scale_type,
+                 uint8_t* q, void* scale, uint8_t* zero);
+/* host: W [N][K] quantised to the nearest code and packed.  asym 0: scale = max|w| / 7, zero must be NULL; asym 1:
+ * scale = (max(w, 0) - min(w, 0)) / 15 with zero points.  Codes are chosen for the scale as rounded. */
+int vela_w4_quantize(const float* W, int N, int K, int group, int asym, int scale_type, uint8_t* q, void* scale, uint8_t* zero);
+
+/* Y[m, n] = sum_k X[m, k] * W[n, k] + bias[n] + residual[m, n] for a few rows (any M; weights are read once for every
+ * 32 rows).  X: bf16, f16, or int8 / e4m3 with xscale [M][ceil(K / xgroup)] (xgroup 64, 128) or [M] (xgroup 0).  int8 rows
+ * are multiplied in integers, exactly, within each group.  bias (float [N]) and residual (Y's type) may be NULL;
+ * residual may be Y itself (with the same ld).  Y: bf16, f16 or f32.  scale_type need not be xtype. */
+int vela_gemv_w4(void* stream, int xtype, const void* X, int ldx, const float* xscale, int xgroup, int M, const vela_w4* W,
+                 const float* bias, const void* residual, int ldr, int ytype, void* Y, int ldy);
+
+/* A mixture-of-experts layer: p = softmax (score 0) or sigmoid (score 1) of X router^T; the topk largest p (+ select_bias,
+ * used for the choice alone) are chosen, ties to the lower expert; their p, divided by their sum where renorm is set, times
+ * `scale`, weigh the experts' outputs down_e (silu(gate_e x) * (up_e x)).
+ * router [E][D] (the activations' type or f32); select_bias float [E] or NULL; E <= 1024, topk <= min(E, 32).
+ * gate_up: E matrices [2 I, D], one after another, I a multiple of 8: rows 16 i .. 16 i + 7 are gate rows 8 i .. 8 i + 7 and
+ * rows 16 i + 8 .. 16 i + 15 the up rows of the same numbers.  down: E matrices [D, I].  Both vela_w4's N, K are one
+ * expert's.  The hidden values are carried as the sum of two bf16 numbers (16 bits of precision). */
+typedef struct vela_moe {
+    int D, I, E, topk;
+    const void* router; int router_type; const float* select_bias;
+    int score, renorm; float scale;
+    vela_w4 gate_up, down;
+} vela_moe;
+/* bytes of workspace for T tokens (0: arguments that vela_moe_w4 refuses).  Its contents need no preparation. */
+size_t vela_moe_w4_workspace(const vela_moe* L, int T);
+/* Y [T, D] = the layer's output for X [T, D] (`type` bf16 or f16).  ids [T][topk] int32 and weights [T][topk] float
+ * (largest first) are written where they are not NULL.  A NaN among a token's scores counts as the smallest score.
+ * workspace: 16-byte aligned; calls that may overlap need one each. */
+int vela_moe_w4(void* stream, int type, const void* X, int ldx, int T, const vela_moe* L, void* Y, int ldy,
+                int32_t* ids, float* weights, void* workspace, size_t workspace_bytes);
+
+/* ---------------------------------------------------------------------------------
  * Engine: one denoising step of the SD-turbo UNet per batch (src/engine.h:16-124).
  * A model holds the prepared weights of one GPU and is shared read-only by its engines; an engine
  * (one per host thread, the reference's "lane") owns a stream, an activation arena and two

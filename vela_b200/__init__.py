@@ -88,6 +88,34 @@ def share_hash(header80, poi32):
     return out.raw
 
 
+def w4_quantize(W, group=128, asym=False, scale_type="bf16"):
+    """4-bit weights of a float matrix [N, K] in the library's layout (vela_w4_quantize): a dict of numpy arrays q, scale
+    (the 16-bit words) and zero (None unless asym), with N, K, group and scale_type (abi.T_BF16 / abi.T_F16), to be copied to the GPU and
+    described by abi.W4."""
+    import numpy as np
+    from . import abi
+    w = np.ascontiguousarray(W, np.float32)
+    if w.ndim != 2:
+        raise ValueError("w4_quantize: a matrix is expected")
+    st = {"bf16": abi.T_BF16, "f16": abi.T_F16}[scale_type]
+    N, K = w.shape
+    n = lib().vela_w4_scales(N, K, int(group))
+    q, s = np.zeros(lib().vela_w4_bytes(N, K), np.uint8), np.zeros(n, np.uint16)
+    z = np.zeros(n, np.uint8) if asym else None
+    p = lambda a: None if a is None else a.ctypes.data_as(ctypes.c_void_p)  # noqa: E731
+    check(lib().vela_w4_quantize(p(w), N, K, int(group), int(bool(asym)), st, p(q), p(s), p(z)))
+    return {"q": q, "scale": s, "zero": z, "N": N, "K": K, "group": int(group), "scale_type": st}
+
+
+def moe_gate_up(gate, up):
+    """The rows of an expert's gate and up matrices [I, D] in the order of vela_moe's gate_up: 8 gate rows, 8 up rows, in turn."""
+    import numpy as np
+    g, u = np.asarray(gate), np.asarray(up)
+    if g.shape != u.shape or g.ndim != 2 or g.shape[0] % 8:
+        raise ValueError("moe_gate_up: two [I, D] matrices of one shape are expected, I a multiple of 8")
+    return np.stack((g.reshape(-1, 8, g.shape[1]), u.reshape(-1, 8, u.shape[1])), 1).reshape(-1, g.shape[1])
+
+
 class Model:
     """Weights of one GPU (vela_model_load): a POISD file prepared for the tcgen05 kernels."""
 

@@ -27,8 +27,20 @@ class AEpi(ctypes.Structure):
                 ("workspace", P), ("workspace_bytes", SZ)]
 
 
+class W4(ctypes.Structure):
+    """vela_w4"""
+    _fields_ = [("q", P), ("scale", P), ("zero", P), ("N", I), ("K", I), ("group", I), ("scale_type", I)]
+
+
+class Moe(ctypes.Structure):
+    """vela_moe"""
+    _fields_ = [("D", I), ("I", I), ("E", I), ("topk", I), ("router", P), ("router_type", I), ("select_bias", P),
+                ("score", I), ("renorm", I), ("scale", ctypes.c_float), ("gate_up", W4), ("down", W4)]
+
+
 SRC_I8, SRC_X32, SRC_CONV32 = 0, 1, 2
 EPI_PLAIN, EPI_SPLIT3, EPI_GEGLU, EPI_GELU, EPI_QKV = 0, 1, 2, 3, 4
+T_BF16, T_F16, T_F32, T_I8, T_E4M3 = 0, 1, 2, 3, 4
 
 SIGNATURES = {
     "vela_last_error": (ctypes.c_char_p, []),
@@ -65,6 +77,14 @@ SIGNATURES = {
     "vela_quant_v_static": (I, [P, P, I, I, I, I, I, P, P, P, P]),
     "vela_fused_attention": (I, [P] + [P] * 13 + [I] * 7 + [P, I, P, P, P, P]),
     "vela_fused_attention_stalled": (I, [P] + [P] * 13 + [I] * 7 + [P, I, P, P, LL]),
+    "vela_rms_norm_q8": (I, [P, I, P, I, P, I, P, ctypes.c_float, I, I, P, I, P, I, I, P, I, P, I]),
+    "vela_w4_bytes": (SZ, [I, I]),
+    "vela_w4_scales": (SZ, [I, I, I]),
+    "vela_w4_pack": (I, [P, P, P, I, I, I, I, P, P, P]),
+    "vela_w4_quantize": (I, [P, I, I, I, I, I, P, P, P]),
+    "vela_gemv_w4": (I, [P, I, P, I, P, I, I, ctypes.POINTER(W4), P, P, I, I, P, I]),
+    "vela_moe_w4_workspace": (SZ, [ctypes.POINTER(Moe), I]),
+    "vela_moe_w4": (I, [P, I, P, I, I, ctypes.POINTER(Moe), P, I, P, P, P, SZ]),
     "vela_model_load": (P, [I, ctypes.c_char_p]),
     "vela_model_load_memory": (P, [I, P, SZ]),
     "vela_model_free": (None, [P]),

@@ -1,0 +1,223 @@
+// Residual addition, root-mean-square norm and 8-bit quantisation of rows in one pass:
+//   h = X + R,  S = h,  y = h * rsqrt(mean(h^2) + eps) * g,  Y = y,  Q = y / scale.
+// h stays in 32-bit registers between the two reductions (the mean square, and the largest |y| of a row or group
+// of columns), so each input is read once and each output written once.
+#include "elem.cuh"
+#include "host_util.h"
+#include "vela_b200.h"
+
+namespace vela {
+namespace {
+
+constexpr float AMAX_MIN = 1e-30f;     // the scale of an all-zero row or group: 127 / AMAX_MIN is still a finite float
+
+struct NormArgs {
+    const void* X; const void* R; const void* g; void* S; void* Y; void* Q; float* qscale;
+    int ldx, ldr, lds, ldy, ldq, M, C, qgroup, ngroups;
+    float eps;
+};
+
+template <int THREADS> __device__ __forceinline__ float block_sum(float v, float* red) {
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (THREADS == 32) return v;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float s = 0.f;
+    for (int i = 0; i < THREADS / 32; ++i) s += red[i];
+    return s;
+}
+template <int THREADS> __device__ __forceinline__ float block_max(float v, float* red) {
+    for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (THREADS == 32) return v;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float s = 0.f;
+    for (int i = 0; i < THREADS / 32; ++i) s = max_nan(s, red[i]);
+    return s;
+}
+
+// 8 values of q = y * inv as bytes
+template <int QT> __device__ __forceinline__ void store_q8(uint8_t* p, int n, bool vec, const float (&y)[8], float inv) {
+    union { uint2 u; uint8_t b[8]; __nv_fp8x2_storage_t h[4]; } o;
+    if constexpr (QT == VELA_T_I8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o.b[i] = uint8_t(max(-127, min(127, __float2int_rn(y[i] * inv))));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o.h[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i] * inv, y[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+    }
+    if (vec) *reinterpret_cast<uint2*>(p) = o.u;
+    else
+#pragma unroll
+        for (int i = 0; i < 8; ++i) if (i < n) p[i] = o.b[i];
+}
+
+// One block of THREADS threads for each row; thread i holds values 8 (i + j THREADS) .. + 7, j < V, in registers.
+// The group of 64 or 128 columns is 8 or 16 neighbouring lanes.
+template <class T, int QT, int THREADS, int V> __global__ void __launch_bounds__(THREADS) rms_norm_kernel(NormArgs a, bool vec) {
+    __shared__ float red[THREADS / 32 + 1];
+    constexpr float TOP = QT == VELA_T_I8 ? 127.f : 448.f;
+    const size_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.X) + row * a.ldx;
+    const T* r = a.R ? static_cast<const T*>(a.R) + row * a.ldr : nullptr;
+    const T* g = static_cast<const T*>(a.g);
+    float h[V][8];
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = 8 * (int(threadIdx.x) + j * THREADS), n = min(8, a.C - c);
+        if (n <= 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[j][i] = 0.f;
+            continue;
+        }
+        load8(x + c, n, vec, h[j]);
+        if (r) {
+            float t[8];
+            load8(r + c, n, vec, t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[j][i] += t[i];
+        }
+        if (a.S) store8(static_cast<T*>(a.S) + row * a.lds + c, n, vec, h[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(h[j][i], h[j][i], ss);
+    }
+    const float rstd = rsqrtf(block_sum<THREADS>(ss, red) / float(a.C) + a.eps);
+    float top = 0.f;
+    float am[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = 8 * (int(threadIdx.x) + j * THREADS), n = min(8, a.C - c);
+        am[j] = 0.f;
+        if (n <= 0) continue;
+        float t[8];
+        load8(g + c, n, vec, t);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { h[j][i] = h[j][i] * rstd * t[i]; if (i < n) am[j] = max_nan(am[j], fabsf(h[j][i])); }
+        if (a.Y) store8(static_cast<T*>(a.Y) + row * a.ldy + c, n, vec, h[j]);
+        top = max_nan(top, am[j]);
+    }
+    if (!a.Q) return;
+    if (a.qgroup == 0) top = block_max<THREADS>(top, red);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = 8 * (int(threadIdx.x) + j * THREADS), n = min(8, a.C - c);
+        float m = top;
+        if (a.qgroup) {
+            m = am[j];
+            for (int o = 1; o < a.qgroup / 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        }
+        if (n <= 0) continue;
+        m = m < AMAX_MIN ? AMAX_MIN : m;
+        if (a.qgroup ? c % a.qgroup == 0 : c == 0) a.qscale[row * a.ngroups + (a.qgroup ? c / a.qgroup : 0)] = m / TOP;
+        store_q8<QT>(static_cast<uint8_t*>(a.Q) + row * a.ldq + c, n, vec, h[j], TOP / m);
+    }
+}
+
+// Rows too long for the registers: the inputs are read again for each step.  S is written last, since it may be X or R.
+template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREADS) rms_norm_long_kernel(NormArgs a, bool vec) {
+    __shared__ float red[THREADS / 32 + 1];
+    constexpr float TOP = QT == VELA_T_I8 ? 127.f : 448.f;
+    const size_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.X) + row * a.ldx;
+    const T* r = a.R ? static_cast<const T*>(a.R) + row * a.ldr : nullptr;
+    const T* g = static_cast<const T*>(a.g);
+    auto get = [&](int c, int n, float (&h)[8]) {
+        load8(x + c, n, vec, h);
+        if (r) {
+            float t[8];
+            load8(r + c, n, vec, t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] += t[i];
+        }
+    };
+    float ss = 0.f;
+    for (int c = 8 * threadIdx.x; c < a.C; c += 8 * THREADS) {
+        float h[8];
+        get(c, min(8, a.C - c), h);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(h[i], h[i], ss);
+    }
+    const float rstd = rsqrtf(block_sum<THREADS>(ss, red) / float(a.C) + a.eps);
+    float top = 0.f;
+    if (a.Q && a.qgroup == 0) {
+        for (int c = 8 * threadIdx.x; c < a.C; c += 8 * THREADS) {
+            float h[8], t[8];
+            const int n = min(8, a.C - c);
+            get(c, n, h);
+            load8(g + c, n, vec, t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) if (i < n) top = max_nan(top, fabsf(h[i] * rstd * t[i]));
+        }
+        top = block_max<THREADS>(top, red);
+    }
+    for (int c0 = 0; c0 < a.C; c0 += 8 * THREADS) {
+        const int c = c0 + 8 * int(threadIdx.x), n = min(8, a.C - c);
+        float h[8], m = 0.f;
+        if (n > 0) {
+            float t[8];
+            get(c, n, h);
+            load8(g + c, n, vec, t);
+            if (a.S) store8(static_cast<T*>(a.S) + row * a.lds + c, n, vec, h);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { h[i] = h[i] * rstd * t[i]; if (i < n) m = max_nan(m, fabsf(h[i])); }
+            if (a.Y) store8(static_cast<T*>(a.Y) + row * a.ldy + c, n, vec, h);
+        }
+        if (!a.Q) continue;
+        if (a.qgroup) { for (int o = 1; o < a.qgroup / 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o)); }
+        else m = top;
+        if (n <= 0) continue;
+        m = m < AMAX_MIN ? AMAX_MIN : m;
+        if (a.qgroup ? c % a.qgroup == 0 : c == 0) a.qscale[row * a.ngroups + (a.qgroup ? c / a.qgroup : 0)] = m / TOP;
+        store_q8<QT>(static_cast<uint8_t*>(a.Q) + row * a.ldq + c, n, vec, h, TOP / m);
+    }
+}
+
+template <class T, int QT> void launch(cudaStream_t st, const NormArgs& a, bool vec) {
+    const int nv = ceil_div(a.C, 8);
+    if (nv <= 128) rms_norm_kernel<T, QT, 128, 1><<<a.M, 128, 0, st>>>(a, vec);
+    else if (nv <= 256) rms_norm_kernel<T, QT, 256, 1><<<a.M, 256, 0, st>>>(a, vec);
+    else if (nv <= 512) rms_norm_kernel<T, QT, 256, 2><<<a.M, 256, 0, st>>>(a, vec);
+    else if (nv <= 1024) rms_norm_kernel<T, QT, 512, 2><<<a.M, 512, 0, st>>>(a, vec);
+    else if (nv <= 2048) rms_norm_kernel<T, QT, 512, 4><<<a.M, 512, 0, st>>>(a, vec);
+    else rms_norm_long_kernel<T, QT, 512><<<a.M, 512, 0, st>>>(a, vec);
+}
+
+void rms_norm_q8(cudaStream_t st, int type, const NormArgs& a, int qtype) {
+    VELA_REQUIRE(type == VELA_T_BF16 || type == VELA_T_F16 || type == VELA_T_F32, "rms_norm_q8: type must be bf16, f16 or f32");
+    VELA_REQUIRE(a.M >= 0 && a.C > 0, "rms_norm_q8: M >= 0 and C > 0");
+    if (a.M == 0) return;
+    VELA_REQUIRE(a.X && a.g, "rms_norm_q8: null X or g");
+    VELA_REQUIRE(a.ldx >= a.C && (!a.R || a.ldr >= a.C) && (!a.S || a.lds >= a.C) && (!a.Y || a.ldy >= a.C) && (!a.Q || a.ldq >= a.C),
+                 "rms_norm_q8: a leading dimension below C");
+    VELA_REQUIRE(a.eps >= 0.f, "rms_norm_q8: eps must not be negative");
+    VELA_REQUIRE(!(a.S && ((a.S == a.X && a.lds != a.ldx) || (a.S == a.R && a.lds != a.ldr))), "rms_norm_q8: S in place needs the same ld");
+    if (a.Q) {
+        VELA_REQUIRE(qtype == VELA_T_I8 || qtype == VELA_T_E4M3, "rms_norm_q8: qtype must be int8 or e4m3");
+        VELA_REQUIRE(a.qscale, "rms_norm_q8: Q without qscale");
+        VELA_REQUIRE(a.qgroup == 0 || a.qgroup == 64 || a.qgroup == 128, "rms_norm_q8: qgroup must be 0, 64 or 128");
+    }
+    const size_t b = elem_bytes(type);
+    for (const void* p : {a.X, a.R, a.g, static_cast<const void*>(a.S), static_cast<const void*>(a.Y)})
+        VELA_REQUIRE(aligned(p, b), "rms_norm_q8: a pointer is not aligned to its type");
+    VELA_REQUIRE(aligned(a.qscale, 4), "rms_norm_q8: qscale is not aligned");
+    auto row16 = [&](const void* p, int ld) { return !p || (aligned(p, 16) && ld * b % 16 == 0); };
+    const bool vec = a.C % 8 == 0 && row16(a.X, a.ldx) && row16(a.R, a.ldr) && row16(a.S, a.lds) && row16(a.Y, a.ldy) && aligned(a.g, 16) &&
+                     (!a.Q || (aligned(a.Q, 8) && a.ldq % 8 == 0));
+    const bool i8 = qtype == VELA_T_I8;
+    if (type == VELA_T_BF16) i8 ? launch<__nv_bfloat16, VELA_T_I8>(st, a, vec) : launch<__nv_bfloat16, VELA_T_E4M3>(st, a, vec);
+    else if (type == VELA_T_F16) i8 ? launch<__half, VELA_T_I8>(st, a, vec) : launch<__half, VELA_T_E4M3>(st, a, vec);
+    else i8 ? launch<float, VELA_T_I8>(st, a, vec) : launch<float, VELA_T_E4M3>(st, a, vec);
+}
+}  // namespace
+}  // namespace vela
+
+extern "C" int vela_rms_norm_q8(void* stream, int type, const void* X, int ldx, const void* R, int ldr, const void* g, float eps, int M, int C,
+                                void* S, int lds, void* Y, int ldy, int qtype, void* Q, int ldq, float* qscale, int qgroup) {
+    return vela::guarded("vela_rms_norm_q8", [&] {
+        vela::NormArgs a{X, R, g, S, Y, Q, qscale, ldx, ldr, lds, ldy, ldq, M, C, qgroup, qgroup > 0 ? (C - 1) / qgroup + 1 : 1, eps};
+        vela::rms_norm_q8(static_cast<cudaStream_t>(stream), type, a, qtype);
+    });
+}
