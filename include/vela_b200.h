@@ -245,6 +245,10 @@ size_t vela_moe_w4_workspace(const vela_moe* L, int T);
  * workspace: 16-byte aligned; calls that may overlap need one each. */
 int vela_moe_w4(void* stream, int type, const void* X, int ldx, int T, const vela_moe* L, void* Y, int ldy,
                 int32_t* ids, float* weights, void* workspace, size_t workspace_bytes);
+/* Failure-path test entry: vela_moe_w4 whose blocks wait at their barrier for one block more than there are, at most
+ * wait_limit_cycles SM clock cycles; they return without the down products and vela_device_error reads non-zero.  Y is left unwritten. */
+int vela_moe_w4_stalled(void* stream, int type, const void* X, int ldx, int T, const vela_moe* L, void* Y, int ldy,
+                        int32_t* ids, float* weights, void* workspace, size_t workspace_bytes, long long wait_limit_cycles);
 
 /* ---------------------------------------------------------------------------------
  * Engine: one denoising step of the SD-turbo UNet per batch (src/engine.h:16-124).

@@ -190,3 +190,20 @@ def test_no_tokens():
     x = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")
     c = layer.c()
     V.check(V.lib().vela_moe_w4(None, abi.T_BF16, None, 64, 0, ctypes.byref(c), None, 64, None, None, None, 0))
+
+
+def test_wait_timeout_then_right():
+    """the grid's barrier waits for a block that does not exist: the call ends by itself, reports, and leaves nothing behind"""
+    layer = Layer(12, 256, 128, 8, 2, abi.T_BF16, 64)
+    x = torch.randn(4, 256, device="cuda").bfloat16()
+    y = torch.full_like(x, 7)
+    c = layer.c()
+    n = V.lib().vela_moe_w4_workspace(ctypes.byref(c), 4)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    assert V.lib().vela_device_error(1) == 0
+    V.check(V.lib().vela_moe_w4_stalled(None, abi.T_BF16, ptr(x), 256, 4, ctypes.byref(c), ptr(y), 256, None, None, ptr(ws), n, 1_000_000))
+    torch.cuda.synchronize()
+    assert V.lib().vela_device_error(1) != 0 and (y == 7).all()
+    layer(x, y, ws=ws)
+    assert V.lib().vela_device_error(1) == 0
+    layer.check(x, y, None, None)

@@ -85,6 +85,7 @@ SIGNATURES = {
     "vela_gemv_w4": (I, [P, I, P, I, P, I, I, ctypes.POINTER(W4), P, P, I, I, P, I]),
     "vela_moe_w4_workspace": (SZ, [ctypes.POINTER(Moe), I]),
     "vela_moe_w4": (I, [P, I, P, I, I, ctypes.POINTER(Moe), P, I, P, P, P, SZ]),
+    "vela_moe_w4_stalled": (I, [P, I, P, I, I, ctypes.POINTER(Moe), P, I, P, P, P, SZ, LL]),
     "vela_model_load": (P, [I, ctypes.c_char_p]),
     "vela_model_load_memory": (P, [I, P, SZ]),
     "vela_model_free": (None, [P]),

@@ -1,8 +1,13 @@
 // Products of a few rows with 4-bit weights: Y[m, n] = sum_k X[m, k] (code - zero) scale + bias + residual.
-// A block of 8 warps takes R row tiles (16 R columns of Y) and 8 NT rows of X; its warps share out the tiles along K
-// and add their sums in shared memory, in the order of the warps.
+//
+// The weights are read once and bound the call, so what counts is to keep enough of them in flight and to spend few
+// instructions on each.  The grid is one wave of 8-warp blocks that stay for the whole call.  Row group (R row tiles) i + j * grid is the j-th of
+// block i, so every SM gets about the same number; 2^ksl warps share out a group's units of 128 columns (unit u goes to warp
+// u mod 2^ksl) and add their sums in shared memory in the order of the warps.  Each warp loads one unit ahead; the many warps of an SM
+// keep the rest in flight.  Activations are read through the L1 cache, which the weights pass by.
 #include "host_util.h"
 #include "w4.cuh"
+#include <algorithm>
 
 namespace vela {
 namespace {
@@ -13,101 +18,145 @@ struct GemvArgs {
     w4::Weights W;
     const void* X; const float* xscale; const float* bias; const void* residual; void* Y;
     int ldx, xgshift, nxg, M, ldr, ldy, ytype;       // xgshift < 0: one scale for each row of X
+    int ksl;                                         // log2 of the warps that share a row group
     bool vec;
 };
 
-template <int XT, int NT, int R, bool G32> __global__ void __launch_bounds__(WARPS * 32) gemv_kernel(GemvArgs a) {
+template <int XT> __device__ __forceinline__ void write_y(const GemvArgs& a, int m, int n, float v) {
+    if (w4::Act<XT>::scaled && a.xgshift < 0) v *= __ldg(a.xscale + m);
+    if (a.bias) v += __ldg(a.bias + n);
+    const size_t at = size_t(m) * a.ldy + n, rat = size_t(m) * a.ldr + n;
+    if (a.ytype == VELA_T_F32) {
+        if (a.residual) v += static_cast<const float*>(a.residual)[rat];
+        static_cast<float*>(a.Y)[at] = v;
+    } else if (a.ytype == VELA_T_BF16) {
+        if (a.residual) v += __bfloat162float(static_cast<const __nv_bfloat16*>(a.residual)[rat]);
+        static_cast<__nv_bfloat16*>(a.Y)[at] = __float2bfloat16_rn(v);
+    } else {
+        if (a.residual) v += __half2float(static_cast<const __half*>(a.residual)[rat]);
+        static_cast<__half*>(a.Y)[at] = __float2half_rn(v);
+    }
+}
+
+__device__ __forceinline__ void group_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(threads) : "memory"); }
+
+template <int XT, int NT, int R, int BLOCKS, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS * 32, BLOCKS) gemv_kernel(const GemvArgs a) {
     typedef typename w4::Act<XT>::X X;
-    constexpr int REGS = w4::Act<XT>::regs;
+    typedef w4::Unit<FOLD, ZERO> Unit;
     __shared__ float red[WARPS][NT * 8][R * 16 + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int rt0 = blockIdx.x * R, m0 = blockIdx.y * NT * 8;
-    const int nrt = (a.W.N + 15) / 16;
-    const X* xr[NT];
+    const int m0 = blockIdx.y * NT * 8;
+    const int nrt = w4::row_tiles(a.W), nrg = (nrt + R - 1) / R, nu = w4::units(a.W);
+    const int ks = 1 << a.ksl, part = warp & (ks - 1), slots = WARPS >> a.ksl, sl = warp >> a.ksl;
+    const w4::Consts k = w4::consts<typename w4::Act<XT>::M>();
+    const X* row[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int m = m0 + 8 * n + g;
-        xr[n] = m < a.M ? static_cast<const X*>(a.X) + size_t(m) * a.ldx : nullptr;
-    }
-    float acc[R][NT][4];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.f;
+    for (int n = 0; n < NT; ++n) row[n] = static_cast<const X*>(a.X) + size_t(min(m0 + 8 * n + g, a.M - 1)) * a.ldx + 8 * t;
 
-    for (int kt = warp; kt < a.W.kt; kt += WARPS) {
-        uint4 w[R];
-        w4::ScaleZero sz[R][2];
+    const int whole = a.vec ? a.W.K >> 7 : 0;              // units that need no care
+
+    for (int rg = blockIdx.x + gridDim.x * sl; rg < nrg; rg += gridDim.x * slots) {
+        float acc[R][NT][4] = {};
+        w4::RowPtr at[R];
+        const X* x[NT];
+        int u = part;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int rt = min(rt0 + r, nrt - 1);
-            w[r] = __ldg(a.W.q + (size_t(rt) * a.W.kt + kt) * 32 + lane);
-            sz[r][0] = w4::load_scale(a.W, rt, kt * 64, g);
-            if constexpr (G32) sz[r][1] = kt * 64 + 32 < a.W.K ? w4::load_scale(a.W, rt, kt * 64 + 32, g) : sz[r][0];
-            else sz[r][1] = sz[r][0];
-        }
-        uint32_t b[2][NT][REGS];
-        float2 sx[NT];
+        for (int r = 0; r < R; ++r) at[r] = w4::row_ptr(a.W, min(rg * R + r, nrt - 1), u, lane);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+        for (int n = 0; n < NT; ++n) x[n] = row[n] + size_t(u) * 128;
+        auto load = [&](Unit (&s)[R]) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int k = kt * 64 + 32 * h + 8 * t;
-                w4::load_half<XT>(b[h][n], xr[n] ? xr[n] + k : nullptr, a.W.K - k, a.vec);
+            for (int r = 0; r < R; ++r) { w4::load_unit(s[r], at[r], a.W); w4::advance(at[r], a.W, ks); }
+        };
+        auto sx = [&](int f, int n) {
+            if (a.xgshift < 0) return make_float2(1.f, 1.f);
+            const int m = m0 + 8 * n + 2 * t, xi = min((u * 128 + f * FOLD) >> a.xgshift, a.nxg - 1);
+            return make_float2(__ldg(a.xscale + size_t(min(m, a.M - 1)) * a.nxg + xi), __ldg(a.xscale + size_t(min(m + 1, a.M - 1)) * a.nxg + xi));
+        };
+        auto work = [&](const Unit (&s)[R]) {
+            w4::unit<XT, true, NT, R>(acc, s, x, 0, a.W.f16, k, sx);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) x[n] += ks * 128;
+            u += ks;
+        };
+        Unit one[R], two[R];
+        if (u < whole) {
+            load(one);
+            while (true) {
+                if (u + ks < whole) load(two);
+                work(one);
+                if (u >= whole) break;
+                if (u + ks < whole) load(one);
+                work(two);
+                if (u >= whole) break;
             }
-            sx[n] = make_float2(1.f, 1.f);
-            if (w4::Act<XT>::scaled && a.xgshift >= 0) {
-                const int m = m0 + 8 * n + 2 * t, i = kt * 64 >> a.xgshift;
-                if (m < a.M) sx[n].x = __ldg(a.xscale + size_t(m) * a.nxg + i);
-                if (m + 1 < a.M) sx[n].y = __ldg(a.xscale + size_t(m + 1) * a.nxg + i);
-            }
         }
-        int ones[2][NT][2];
-        w4::sums<XT, NT>(ones, b);
+        for (; u < nu; u += ks) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) w4::tile<XT, NT, G32>(acc[r], w[r], b, ones, sz[r], sx, a.W.f16);
-    }
+            for (int r = 0; r < R; ++r) { w4::load_last(one[r], at[r], a.W, u); w4::advance(at[r], a.W, ks); }
+            w4::unit<XT, false, NT, R>(acc, one, x, a.W.K - u * 128 - 8 * t, a.W.f16, k, sx);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+            for (int n = 0; n < NT; ++n) x[n] += ks * 128;
+        }
+        if (ks == 1) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) red[warp][8 * n + 2 * t + (i & 1)][16 * r + g + 8 * (i >> 1)] = acc[r][n][i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < NT * 8 * R * 16; i += WARPS * 32) {
-        const int c = i % (R * 16), mm = i / (R * 16), n = rt0 * 16 + c, m = m0 + mm;
-        if (n >= a.W.N || m >= a.M) continue;
-        float v = 0.f;
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) v += red[w][mm][c];
-        if (w4::Act<XT>::scaled && a.xgshift < 0) v *= __ldg(a.xscale + m);
-        if (a.bias) v += __ldg(a.bias + n);
-        const size_t at = size_t(m) * a.ldy + n, rat = size_t(m) * a.ldr + n;
-        if (a.ytype == VELA_T_F32) {
-            if (a.residual) v += static_cast<const float*>(a.residual)[rat];
-            static_cast<float*>(a.Y)[at] = v;
-        } else if (a.ytype == VELA_T_BF16) {
-            if (a.residual) v += __bfloat162float(static_cast<const __nv_bfloat16*>(a.residual)[rat]);
-            static_cast<__nv_bfloat16*>(a.Y)[at] = __float2bfloat16_rn(v);
+                    for (int i = 0; i < 4; ++i) {
+                        const int m = m0 + 8 * n + 2 * t + (i & 1), c = (rg * R + r) * 16 + g + 8 * (i >> 1);
+                        if (m < a.M && c < a.W.N) write_y<XT>(a, m, c, acc[r][n][i]);
+                    }
         } else {
-            if (a.residual) v += __half2float(static_cast<const __half*>(a.residual)[rat]);
-            static_cast<__half*>(a.Y)[at] = __float2half_rn(v);
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) red[warp][8 * n + 2 * t + (i & 1)][16 * r + g + 8 * (i >> 1)] = acc[r][n][i];
+            group_sync(1 + sl, ks * 32);
+            const int rows = min(NT * 8, a.M - m0);
+            for (int i = part * 32 + lane; i < rows * (R * 16); i += ks * 32) {
+                const int c = i % (R * 16), mm = i / (R * 16);
+                float v = 0.f;
+                for (int w = 0; w < ks; ++w) v += red[sl * ks + w][mm][c];
+                if (rg * R * 16 + c < a.W.N) write_y<XT>(a, m0 + mm, rg * R * 16 + c, v);
+            }
+            group_sync(1 + sl, ks * 32);
         }
     }
 }
 
-template <int XT, int NT, int R> void launch(cudaStream_t st, const GemvArgs& a) {
-    const dim3 grid(ceil_div(ceil_div(a.W.N, 16), R), ceil_div(a.M, 8 * NT));
-    VELA_REQUIRE(grid.y <= 65535u, "gemv_w4: too many rows");
-    if (a.W.gshift == 5) gemv_kernel<XT, NT, R, true><<<grid, WARPS * 32, 0, st>>>(a);
-    else gemv_kernel<XT, NT, R, false><<<grid, WARPS * 32, 0, st>>>(a);
+template <int XT, int NT, int R, int BLOCKS, int FOLD, bool ZERO> void launch(cudaStream_t st, GemvArgs a) {
+    auto* kernel = gemv_kernel<XT, NT, R, BLOCKS, FOLD, ZERO>;
+    const int nrg = ceil_div(w4::row_tiles(a.W), R), nu = w4::units(a.W), mb = ceil_div(a.M, 8 * NT);
+    VELA_REQUIRE(mb <= 65535, "gemv_w4: too many rows");
+    const int wave = std::max(1, sm_count() * blocks_per_sm(reinterpret_cast<const void*>(kernel), WARPS * 32, 0) / mb);
+    const dim3 grid(std::min(nrg, wave), mb);
+    // as many warps on a row group as the block has left over, each with a unit at least
+    const int per = ceil_div(nrg, int(grid.x));
+    a.ksl = 0;
+    while (a.ksl < 3 && (per << (a.ksl + 1)) <= WARPS && nu >= (1 << (a.ksl + 1))) ++a.ksl;
+    kernel<<<grid, WARPS * 32, 0, st>>>(a);
+}
+template <int XT, int NT, int R, int BLOCKS> void launch(cudaStream_t st, const GemvArgs& a) {
+    const int fold = a.W.gshift == 5 ? 32 : a.W.gshift == 6 || a.xgshift == 6 ? 64 : 128;
+    if (a.W.zero) {
+        if (fold == 32) launch<XT, NT, R, BLOCKS, 32, true>(st, a);
+        else if (fold == 64) launch<XT, NT, R, BLOCKS, 64, true>(st, a);
+        else launch<XT, NT, R, BLOCKS, 128, true>(st, a);
+    } else {
+        if (fold == 32) launch<XT, NT, R, BLOCKS, 32, false>(st, a);
+        else if (fold == 64) launch<XT, NT, R, BLOCKS, 64, false>(st, a);
+        else launch<XT, NT, R, BLOCKS, 128, false>(st, a);
+    }
 }
 template <int XT> void launch(cudaStream_t st, const GemvArgs& a) {
-    if (a.M <= 8) launch<XT, 1, 1>(st, a);
-    else if (a.M <= 16) launch<XT, 2, 1>(st, a);
-    else launch<XT, 4, 1>(st, a);
+    if (a.M <= 8) launch<XT, 1, 1, 4>(st, a);
+    else if (a.M <= 16) launch<XT, 2, 2, 2>(st, a);
+    else if (a.M <= 24) launch<XT, 3, 1, 2>(st, a);
+    else launch<XT, 4, 1, 2>(st, a);
 }
 
 void gemv_w4(cudaStream_t st, int xtype, GemvArgs a, int xgroup) {
@@ -127,7 +176,7 @@ void gemv_w4(cudaStream_t st, int xtype, GemvArgs a, int xgroup) {
         VELA_REQUIRE(xgroup == 0 || xgroup == 64 || xgroup == 128, "gemv_w4: xgroup must be 0, 64 or 128");
         if (xgroup) { a.xgshift = xgroup == 64 ? 6 : 7; a.nxg = (a.W.K - 1) / xgroup + 1; }
     }
-    a.vec = a.W.K % 8 == 0 && a.ldx % 8 == 0 && aligned(a.X, 8 * xb);
+    a.vec = a.ldx % 8 == 0 && aligned(a.X, 8 * xb);
     if (xtype == VELA_T_BF16) launch<VELA_T_BF16>(st, a);
     else if (xtype == VELA_T_F16) launch<VELA_T_F16>(st, a);
     else if (xtype == VELA_T_I8) launch<VELA_T_I8>(st, a);

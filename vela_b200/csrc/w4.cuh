@@ -1,17 +1,16 @@
-// 4-bit weight tiles on the tensor cores: the 16 x 64 tile of vela_w4 (512 bytes, 16 per lane) against up to
-// 8 NT activation rows.
+// 4-bit weight tiles on the tensor cores: the 16 x 64 tile of vela_w4 (512 bytes, 16 per lane) against up to 8 NT
+// activation rows.
 //
 // Lane 4 g + t of a warp holds, in word j (j < 4) of its 16 bytes, rows g and g + 8 at the four columns
-// k = 32 (j / 2) + 8 t + 4 (j % 2) + {0, 1, 2, 3}.  A product over k does not mind in which order k runs, so those
-// columns stand in the places that the instruction numbers 2t, 2t + 1, 2t + 8, 2t + 9 (16-bit operands) or 4t .. 4t + 3
-// (8-bit ones), for the weights and the activations alike: each lane reads 8 neighbouring activations at a time, and
-// the codes come out of a word by masks.  With words w0..w3 of nibbles 0..7, nibbles (0, 4) and (2, 6) are row g's,
-// (1, 5) and (3, 7) row g + 8's column pairs (0, 1) and (2, 3).
+// k = 32 (j / 2) + 8 t + 4 (j % 2) + {0, 1, 2, 3}.  A product over k does not mind in which order k runs, so those columns stand in
+// the places that the instruction numbers 2t, 2t + 1, 2t + 8, 2t + 9 (16-bit operands) or 4t .. 4t + 3 (8-bit ones), for
+// the weights and the activations alike.  Of a word's nibbles 0..7, (0, 4) and (2, 6) are row g's column pairs (0, 1) and (2, 3),
+// (1, 5) and (3, 7) row g + 8's.
 //
-// 16-bit operands: 0x4300 | n is the bf16 number 128 + n and 0x6400 | n the f16 number 1024 + n, from which 128 + zero
-// (1024 + zero) is taken exactly, so the operand is the integer code - zero and no rounding happens before the 32-bit
-// accumulation.  8-bit operands: the codes go in as unsigned bytes, and zero times the sum of the activations
-// (one more product, by ones) is taken off the 32-bit integer sum.
+// 16-bit operands: 0x4300 | n is the bf16 number 128 + n and 0x6400 | n the f16 number 1024 + n (0x5400 | n << 4 the number 64 + n, which
+// saves a shift), from which 128 + zero (1024 + zero, 64 + zero) is taken exactly: the operand is the integer code - zero, and nothing is
+// rounded before the 32-bit accumulation.  8-bit operands: a mask leaves the unsigned byte code (row g) or 16 * code (row g + 8), and zero
+// times the sum of the activations, from one more product by ones, is taken off the 32-bit integer sum.
 #pragma once
 #include "elem.cuh"
 #include "vela_b200.h"
@@ -19,42 +18,64 @@
 namespace vela {
 namespace w4 {
 
-constexpr int TILE_ROWS = 16, TILE_K = 64, TILE_BYTES = 512;
-
-struct Weights {                     // one matrix on the device
+struct Weights {                     // one matrix (or several, one after another) on the device
     const uint4* q; const uint32_t* scale; const uint16_t* zero;     // scale, zero: pairs (row g, row g + 8)
     int N, K, kt, ng, gshift;        // kt: tiles along K; ng: groups; gshift: log2(group)
     bool f16;                        // scale type
 };
+__host__ __device__ __forceinline__ int row_tiles(const Weights& W) { return (W.N + 15) >> 4; }
+__host__ __device__ __forceinline__ int units(const Weights& W) { return (W.kt + 1) >> 1; }
 
-__device__ __forceinline__ void mma_f32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_f32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
+template <class M> struct Ops;      // M: the operands' type
+template <> struct Ops<__nv_bfloat16> {
+    static constexpr uint32_t base0 = 0x43004300u, base1 = 0x43004300u;      // of rows g and g + 8
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+        __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+        return *reinterpret_cast<uint32_t*>(&r);
+    }
+    static __device__ __forceinline__ uint32_t high(uint32_t u, uint32_t, uint32_t m, uint32_t k) { return and_or(u >> 4, m, k); }
+    static __device__ __forceinline__ uint32_t and_or(uint32_t u, uint32_t m, uint32_t k) {
+        uint32_t d;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(u), "r"(m), "r"(k));
+        return d;
+    }
+    static constexpr uint32_t zstep1 = 1;                  // what a step of the zero point adds to the number's bits
+};
+template <> struct Ops<__half> {
+    static constexpr uint32_t base0 = 0x64006400u, base1 = 0x54005400u;
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+        __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+        return *reinterpret_cast<uint32_t*>(&r);
+    }
+    static __device__ __forceinline__ uint32_t high(uint32_t u, uint32_t m4, uint32_t, uint32_t k) { return Ops<__nv_bfloat16>::and_or(u, m4, k); }
+    static __device__ __forceinline__ uint32_t and_or(uint32_t u, uint32_t m, uint32_t k) { return Ops<__nv_bfloat16>::and_or(u, m, k); }
+    static constexpr uint32_t zstep1 = 16;
+};
 __device__ __forceinline__ void mma_i8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <class T> struct Magic;
-template <> struct Magic<__nv_bfloat16> {
-    static constexpr uint32_t bits = 0x43004300u, one = 0x00010001u, base = 0x43004300u;
-    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-        __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-        return *reinterpret_cast<uint32_t*>(&r);
-    }
-};
-template <> struct Magic<__half> {
-    static constexpr uint32_t bits = 0x64006400u, one = 0x00010001u, base = 0x64006400u;
-    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-        __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-        return *reinterpret_cast<uint32_t*>(&r);
-    }
-};
+// Masks and bases in registers that the compiler does not see through: an instruction takes one constant at most, so as constants
+// the mask and the base would cost a second instruction for each operand.
+struct Consts { uint32_t m, m4, k0, k1; };
+template <class M> __device__ __forceinline__ Consts consts() {
+    Consts c;
+    asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(c.m));
+    asm volatile("mov.b32 %0, 0x00f000f0;" : "=r"(c.m4));
+    asm volatile("mov.b32 %0, %1;" : "=r"(c.k0) : "n"(Ops<M>::base0));
+    asm volatile("mov.b32 %0, %1;" : "=r"(c.k1) : "n"(Ops<M>::base1));
+    return c;
+}
+template <> __device__ __forceinline__ Consts consts<int8_t>() { return Consts{}; }
 
 // the pair (row g, row g + 8) of scales as floats
 __device__ __forceinline__ float2 scale_pair(uint32_t u, bool f16) {
@@ -62,27 +83,73 @@ __device__ __forceinline__ float2 scale_pair(uint32_t u, bool f16) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 
-// Activation types.  X: what lies in memory; M: the operand type of the product.  `half` loads the 8 activations of a
-// lane in one half tile as the registers of its two products' second operands.
-template <int XT> struct Act;
-template <> struct Act<VELA_T_BF16> {
-    typedef __nv_bfloat16 X; typedef __nv_bfloat16 M; static constexpr bool scaled = false, integer = false; static constexpr int regs = 4;
-};
-template <> struct Act<VELA_T_F16> {
-    typedef __half X; typedef __half M; static constexpr bool scaled = false, integer = false; static constexpr int regs = 4;
-};
-template <> struct Act<VELA_T_E4M3> {
-    typedef uint8_t X; typedef __half M; static constexpr bool scaled = true, integer = false; static constexpr int regs = 4;
-};
-template <> struct Act<VELA_T_I8> {
-    typedef uint8_t X; typedef int8_t M; static constexpr bool scaled = true, integer = true; static constexpr int regs = 2;
+// weights pass through once: they leave the L1 cache to others
+__device__ __forceinline__ uint4 load_tile(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// A unit is two neighbouring tiles (128 columns) of one row tile: what a warp loads at once.  FOLD (32, 64 or 128) is the
+// number of columns between scalings, the smaller of the weights' and the activations' group; a unit has one scale (and zero) for each fold.
+template <int FOLD, bool ZERO> struct Unit {
+    uint4 w[2];
+    uint32_t s[128 / FOLD];
+    uint32_t z[ZERO ? 128 / FOLD : 1];
 };
 
-// p[0 .. n) with zeros beyond, n <= 8 (may be negative); p null: zeros
-template <int XT> __device__ __forceinline__ void load_half(uint32_t (&b)[Act<XT>::regs], const typename Act<XT>::X* p, int n, bool vec) {
+// Where a unit of one row tile lies for one lane.
+struct RowPtr { const uint4* q; const uint32_t* s; const uint16_t* z; };
+__device__ __forceinline__ RowPtr row_ptr(const Weights& W, size_t rt, int u, int lane) {
+    const size_t grp = rt * W.ng + (size_t(u) << (7 - W.gshift));
+    RowPtr p;
+    p.q = W.q + (rt * W.kt + 2 * size_t(u)) * 32 + lane;
+    p.s = W.scale + grp * 8 + (lane >> 2);
+    p.z = W.zero + grp * 8 + (lane >> 2);
+    return p;
+}
+// `n` units on
+__device__ __forceinline__ void advance(RowPtr& p, const Weights& W, int n) {
+    p.q += n * 64;
+    p.s += (n << (7 - W.gshift)) * 8;
+    p.z += (n << (7 - W.gshift)) * 8;
+}
+template <int FOLD, bool ZERO> __device__ __forceinline__ void load_unit(Unit<FOLD, ZERO>& o, const RowPtr& p, const Weights& W) {
+    o.w[0] = load_tile(p.q);
+    o.w[1] = load_tile(p.q + 32);
+#pragma unroll
+    for (int f = 0; f < 128 / FOLD; ++f) {
+        const int grp = FOLD == 64 ? (f * FOLD) >> W.gshift : f;      // FOLD 32 and 128 are the weights' own groups
+        o.s[f] = __ldg(p.s + grp * 8);
+        if constexpr (ZERO) o.z[f] = __ldg(p.z + grp * 8);
+    }
+}
+// The last unit (number u) may lack its second tile or its last groups: the last tile and group are read again in their
+// place, and meet activations of zero.
+template <int FOLD, bool ZERO> __device__ __forceinline__ void load_last(Unit<FOLD, ZERO>& o, const RowPtr& p, const Weights& W, int u) {
+    o.w[0] = load_tile(p.q);
+    o.w[1] = load_tile(p.q + (2 * u + 1 < W.kt ? 32 : 0));
+    const int left = W.ng - 1 - (u << (7 - W.gshift));
+#pragma unroll
+    for (int f = 0; f < 128 / FOLD; ++f) {
+        const int grp = min((f * FOLD) >> W.gshift, left);
+        o.s[f] = __ldg(p.s + grp * 8);
+        if constexpr (ZERO) o.z[f] = __ldg(p.z + grp * 8);
+    }
+}
+
+// Activation types.  X: what lies in memory; M: the operands' type; REGS: a lane's registers for the 8 columns that it takes of 32.
+template <int XT> struct Act;
+template <> struct Act<VELA_T_BF16> { typedef __nv_bfloat16 X; typedef __nv_bfloat16 M; static constexpr bool scaled = false, integer = false; static constexpr int REGS = 4; };
+template <> struct Act<VELA_T_F16> { typedef __half X; typedef __half M; static constexpr bool scaled = false, integer = false; static constexpr int REGS = 4; };
+template <> struct Act<VELA_T_E4M3> { typedef uint8_t X; typedef __half M; static constexpr bool scaled = true, integer = false; static constexpr int REGS = 4; };
+template <> struct Act<VELA_T_I8> { typedef uint8_t X; typedef int8_t M; static constexpr bool scaled = true, integer = true; static constexpr int REGS = 2; };
+
+// A lane's 8 activations p[0 .. 8) of a 32-column part as operands.  Not WHOLE: n of them exist (may be negative), zeros stand for the others,
+// and p has its type's alignment only.
+template <int XT, bool WHOLE> __device__ __forceinline__ void load_x8(uint32_t (&b)[Act<XT>::REGS], const typename Act<XT>::X* p, int n) {
     if constexpr (sizeof(typename Act<XT>::X) == 2) {
-        if (!p || n <= 0) { b[0] = b[1] = b[2] = b[3] = 0u; return; }
-        if (vec) {
+        if constexpr (WHOLE) {
             const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
             b[0] = u.x; b[1] = u.y; b[2] = u.z; b[3] = u.w;
         } else {
@@ -95,12 +162,10 @@ template <int XT> __device__ __forceinline__ void load_half(uint32_t (&b)[Act<XT
         }
     } else {
         uint2 u = make_uint2(0u, 0u);
-        if (p && n > 0) {
-            if (vec) u = __ldg(reinterpret_cast<const uint2*>(p));
-            else {
+        if constexpr (WHOLE) u = __ldg(reinterpret_cast<const uint2*>(p));
+        else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { if (i < n) u.x |= uint32_t(p[i]) << (8 * i); if (i + 4 < n) u.y |= uint32_t(p[i + 4]) << (8 * i); }
-            }
+            for (int i = 0; i < 4; ++i) { if (i < n) u.x |= uint32_t(p[i]) << (8 * i); if (i + 4 < n) u.y |= uint32_t(p[i + 4]) << (8 * i); }
         }
         if constexpr (XT == VELA_T_I8) {         // bytes in the order of a word's codes: columns 0, 2, 1, 3
             b[0] = __byte_perm(u.x, 0u, 0x3120);
@@ -116,120 +181,224 @@ template <int XT> __device__ __forceinline__ void load_half(uint32_t (&b)[Act<XT
     }
 }
 
-// One half tile (words u0, u1 = 32 columns) of 16 rows against 8 activation rows, added to c; zz: 128 + zero as bf16
-// pairs (1024 + zero as f16 pairs) of rows g and g + 8.
-template <class M> __device__ __forceinline__ void decode16(uint32_t (&a)[4], uint32_t u, uint32_t z0, uint32_t z1) {
-    constexpr uint32_t m = 0x000f000fu, b = Magic<M>::bits;
-    a[0] = Magic<M>::sub((u & m) | b, z0);
-    a[1] = Magic<M>::sub(((u >> 4) & m) | b, z1);
-    a[2] = Magic<M>::sub(((u >> 8) & m) | b, z0);
-    a[3] = Magic<M>::sub(((u >> 12) & m) | b, z1);
-}
-
-// The running product of R row tiles with 8 NT activation rows.  c0, c1: row g, activation rows 2t and 2t + 1; c2, c3: row g + 8.
-template <int XT, int NT, int R> struct Acc {
-    float v[R][NT][4];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[r][n][i] = 0.f;
-    }
-};
-
-struct ScaleZero { uint32_t s; uint32_t z; };
-__device__ __forceinline__ ScaleZero load_scale(const Weights& W, int rt, int k, int g) {
-    const size_t i = (size_t(rt) * W.ng + (k >> W.gshift)) * 8 + g;
-    ScaleZero r;
-    r.s = __ldg(W.scale + i);
-    r.z = W.zero ? __ldg(W.zero + i) : 0x0808u;
-    return r;
-}
-
-// Adds one 64-column tile of row tile r to acc.  b: the activations' operands [half][NT].  sx (8-bit activations): the
-// scales of activation rows 2t, 2t + 1.  G32: groups of 32 columns, so each half has its own scales.
-template <int XT, int NT, bool G32>
-__device__ __forceinline__ void tile(float (&acc)[NT][4], const uint4& w, const uint32_t (&b)[2][NT][Act<XT>::regs], const int (&ones)[2][NT][2],
-                                     const ScaleZero (&sz)[2], const float2 (&sx)[NT], bool f16) {
+// Adds one unit of R row tiles to acc: c0, c1 = row g and activation rows 2t, 2t + 1; c2, c3 = row g + 8.  x[n]: this lane's place (row g of column
+// tile n, column 8 t of the unit; any row where there is none: its column of the product is not used); WHOLE: all 128 columns exist and x is aligned
+// to 8 of them, else left columns exist from x on; sx(f, n): the scales of activation rows 2t, 2t + 1 of column tile n in fold f (8-bit forms).
+template <int XT, bool WHOLE, int NT, int R, int FOLD, bool ZERO, class SX>
+__device__ __forceinline__ void unit(float (&acc)[R][NT][4], const Unit<FOLD, ZERO> (&W)[R], const typename Act<XT>::X* const (&x)[NT], int left, bool f16,
+                                     const Consts& k, SX sx) {
     typedef typename Act<XT>::M M;
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    if constexpr (Act<XT>::integer) {
-        int c[NT][4];
+    constexpr int HALVES = FOLD / 32;
+    constexpr bool AHEAD = NT == 1;                        // all of the unit's activations at once, where the registers allow
+    uint32_t all[AHEAD ? 4 : 1][NT][Act<XT>::REGS];
+    if constexpr (AHEAD) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (G32 || h == 0) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0;
-            }
-            constexpr uint32_t m = 0x0f0f0f0fu;
-            const uint32_t a0 = u[2 * h] & m, a1 = (u[2 * h] >> 4) & m, a2 = u[2 * h + 1] & m, a3 = (u[2 * h + 1] >> 4) & m;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_i8(c[n], a0, a1, a2, a3, b[h][n][0], b[h][n][1]);
-            if (G32 || h == 1) {
-                const ScaleZero q = sz[G32 ? h : 0];
-                const float2 s = scale_pair(q.s, f16);
-                const int z0 = q.z & 0xff, z1 = q.z >> 8;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int t0 = ones[h][n][0] + (G32 ? 0 : ones[0][n][0]), t1 = ones[h][n][1] + (G32 ? 0 : ones[0][n][1]);
-                    acc[n][0] = fmaf(s.x * sx[n].x, float(c[n][0] - z0 * t0), acc[n][0]);
-                    acc[n][1] = fmaf(s.x * sx[n].y, float(c[n][1] - z0 * t1), acc[n][1]);
-                    acc[n][2] = fmaf(s.y * sx[n].x, float(c[n][2] - z1 * t0), acc[n][2]);
-                    acc[n][3] = fmaf(s.y * sx[n].y, float(c[n][3] - z1 * t1), acc[n][3]);
-                }
-            }
-        }
-    } else {
-        float c[NT][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (G32 || h == 0) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-            }
-            const ScaleZero q = sz[G32 ? h : 0];
-            // 128 + zero (1024 + zero) lies zero steps above the base, in both halves of the pair
-            const uint32_t z0 = Magic<M>::base + Magic<M>::one * (q.z & 0xff), z1 = Magic<M>::base + Magic<M>::one * (q.z >> 8);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                uint32_t a[4];
-                decode16<M>(a, u[2 * h + j], z0, z1);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f32(c[n], a, b[h][n][2 * j], b[h][n][2 * j + 1], M());
-            }
-            if (G32 || h == 1) {
-                const float2 s = scale_pair(q.s, f16);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    if constexpr (Act<XT>::scaled) {
-                        acc[n][0] = fmaf(s.x * sx[n].x, c[n][0], acc[n][0]);
-                        acc[n][1] = fmaf(s.x * sx[n].y, c[n][1], acc[n][1]);
-                        acc[n][2] = fmaf(s.y * sx[n].x, c[n][2], acc[n][2]);
-                        acc[n][3] = fmaf(s.y * sx[n].y, c[n][3], acc[n][3]);
-                    } else {
-                        acc[n][0] = fmaf(s.x, c[n][0], acc[n][0]);
-                        acc[n][1] = fmaf(s.x, c[n][1], acc[n][1]);
-                        acc[n][2] = fmaf(s.y, c[n][2], acc[n][2]);
-                        acc[n][3] = fmaf(s.y, c[n][3], acc[n][3]);
-                    }
-                }
-            }
-        }
+        for (int h = 0; h < 4; ++h) load_x8<XT, WHOLE>(all[h][0], x[0] + 32 * h, left - 32 * h);
     }
-}
-
-// sums of the integer activations of one half tile for activation rows 2t, 2t + 1
-template <int XT, int NT> __device__ __forceinline__ void sums(int (&ones)[2][NT][2], const uint32_t (&b)[2][NT][Act<XT>::regs]) {
-    if constexpr (Act<XT>::integer) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+    for (int f = 0; f < 128 / FOLD; ++f) {
+        float d[R][NT][4];
+        float2 tot[NT];                                    // integer forms: sums of activation rows 2t, 2t + 1
+        if constexpr (Act<XT>::integer) {
+            int c[R][NT][4] = {}, s[NT][4] = {};
+#pragma unroll
+            for (int h = f * HALVES; h < (f + 1) * HALVES; ++h) {
+                uint32_t b[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if constexpr (AHEAD) { b[n][0] = all[h][n][0]; b[n][1] = all[h][n][1]; }
+                    else load_x8<XT, WHOLE>(b[n], x[n] + 32 * h, left - 32 * h);
+                    mma_i8(s[n], 0x01010101u, 0u, 0x01010101u, 0u, b[n][0], b[n][1]);
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const uint4 v = W[r].w[h >> 1];
+                    const uint32_t u0 = h & 1 ? v.z : v.x, u1 = h & 1 ? v.w : v.y;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_i8(c[r][n], u0 & 0x0f0f0f0fu, u0 & 0xf0f0f0f0u, u1 & 0x0f0f0f0fu, u1 & 0xf0f0f0f0u, b[n][0], b[n][1]);
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                int c[4] = {0, 0, 0, 0};
-                mma_i8(c, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, b[h][n][0], b[h][n][1]);
-                ones[h][n][0] = c[0]; ones[h][n][1] = c[1];
+                tot[n] = make_float2(float(s[n][0]), float(s[n][1]));
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float z0 = ZERO ? float(W[r].z[ZERO ? f : 0] & 0xffu) : 8.f, z1 = ZERO ? float(W[r].z[ZERO ? f : 0] >> 8) : 8.f;
+                    // exact: all of these are integers (or sixteenths) below 2^24
+                    d[r][n][0] = fmaf(-z0, tot[n].x, float(c[r][n][0])); d[r][n][1] = fmaf(-z0, tot[n].y, float(c[r][n][1]));
+                    d[r][n][2] = fmaf(0.0625f, float(c[r][n][2]), -z1 * tot[n].x); d[r][n][3] = fmaf(0.0625f, float(c[r][n][3]), -z1 * tot[n].y);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) d[r][n][0] = d[r][n][1] = d[r][n][2] = d[r][n][3] = 0.f;
+            uint32_t z0[R], z1[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {      // the number above, with the zero point added to its bits, in both halves
+                const uint32_t z = ZERO ? W[r].z[ZERO ? f : 0] : 0x0808u;
+                z0[r] = Ops<M>::base0 + 0x00010001u * (z & 0xffu);
+                z1[r] = Ops<M>::base1 + 0x00010001u * Ops<M>::zstep1 * (z >> 8);
+            }
+#pragma unroll
+            for (int h = f * HALVES; h < (f + 1) * HALVES; ++h) {
+                uint32_t b[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if constexpr (AHEAD) { b[n][0] = all[h][n][0]; b[n][1] = all[h][n][1]; b[n][2] = all[h][n][2]; b[n][3] = all[h][n][3]; }
+                    else load_x8<XT, WHOLE>(b[n], x[n] + 32 * h, left - 32 * h);
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const uint4 v = W[r].w[h >> 1];
+                        const uint32_t u = h & 1 ? (j ? v.w : v.z) : (j ? v.y : v.x), u8 = u >> 8;
+                        const uint32_t a[4] = {Ops<M>::sub(Ops<M>::and_or(u, k.m, k.k0), z0[r]), Ops<M>::sub(Ops<M>::high(u, k.m4, k.m, k.k1), z1[r]),
+                                               Ops<M>::sub(Ops<M>::and_or(u8, k.m, k.k0), z0[r]), Ops<M>::sub(Ops<M>::high(u8, k.m4, k.m, k.k1), z1[r])};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) Ops<M>::mma(d[r][n], a, b[n][2 * j], b[n][2 * j + 1]);
+                    }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float2 s = scale_pair(W[r].s[f], f16);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float2 p = make_float2(s.x, s.x), q = make_float2(s.y, s.y);
+                if constexpr (Act<XT>::scaled) {
+                    const float2 e = sx(f, n);
+                    p = make_float2(s.x * e.x, s.x * e.y); q = make_float2(s.y * e.x, s.y * e.y);
+                }
+                acc[r][n][0] = fmaf(p.x, d[r][n][0], acc[r][n][0]);
+                acc[r][n][1] = fmaf(p.y, d[r][n][1], acc[r][n][1]);
+                acc[r][n][2] = fmaf(q.x, d[r][n][2], acc[r][n][2]);
+                acc[r][n][3] = fmaf(q.y, d[r][n][3], acc[r][n][3]);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- staged activations
+// Rows of f16 values that were brought into a form in which a weight costs less, once, by whoever produces them: whole units (zeros
+// beyond K), and for each fold of a unit a pair {factor that the staged values have lost, sum of the staged values}.  The bits of a
+// nibble at the bottom of a 16-bit half are, as they stand, the (subnormal) f16 number code * 2^-24, four bits up code * 2^-20, both
+// exact and taken by the tensor cores at full rate: a word takes one shift and four masks (f16 operands as above: 9, bf16: 11), and zero times the sum
+// is taken off the sum of products.
+
+// Brings columns 4 lane .. 4 lane + 3 of a unit (n of them exist) of a row of X to `out` (the unit's 128 values), a warp together; lane 0
+// of each fold writes its pair.
+template <class X, int FOLD> __device__ __forceinline__ void stage_unit(const X* p, int n, __half* out, float2* pair, int lane) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? Elem<X>::get(p[i]) : 0.f;
+    float back = 1.f;
+    if constexpr (Elem<X>::code != VELA_T_F16) {
+        // The largest value is brought into [2^14, 2^15) by a power of two: bf16's 8 bits then fit f16 exactly down to 2^-31 of it, and
+        // what is smaller is rounded to 2^-39 of it, below a 32-bit sum's own rounding.
+        const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(__float_as_uint(v[0]) & 0x7fffffffu, __float_as_uint(v[1]) & 0x7fffffffu),
+                                                                max(__float_as_uint(v[2]) & 0x7fffffffu, __float_as_uint(v[3]) & 0x7fffffffu)));
+        int e = int(top >> 23) - 127;                      // 128: an infinity or a NaN, which stays one
+        e = e > 127 ? 127 : e < -100 ? -100 : e;           // both factors are normal floats
+        const float fwd = __uint_as_float(uint32_t(127 + 14 - e) << 23);
+        back = __uint_as_float(uint32_t(127 - 14 + e) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] *= fwd;
+    }
+    const __half2 lo = __floats2half2_rn(v[0], v[1]), hi = __floats2half2_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(out + 4 * lane) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    const float2 fl = __half22float2(lo), fh = __half22float2(hi);
+    float sum = (fl.x + fl.y) + (fh.x + fh.y);
+#pragma unroll
+    for (int o = 1; o < FOLD / 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane % (FOLD / 4) == 0) pair[lane / (FOLD / 4)] = make_float2(back, sum);
+}
+
+// Adds a unit of one row tile to acc.  x[n]: this lane's place in column tile n (row g, column 8 t of the unit); pair[n][i]: the unit's first pair of
+// activation row 2t + i; nt: the column tiles that hold any row.
+template <int NT, int FOLD, bool ZERO>
+__device__ __forceinline__ void unit_staged(float (&acc)[NT][4], const Unit<FOLD, ZERO>& W, const __half* const (&x)[NT], const float2* const (&pair)[NT][2], int nt, bool f16) {
+    constexpr int HALVES = FOLD / 32;
+    uint4 b[NT][4];
+    float2 pr[NT][2][128 / FOLD];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+        if (n == 0 || n < nt) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) b[n][h] = __ldg(reinterpret_cast<const uint4*>(x[n] + 32 * h));
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int f = 0; f < 128 / FOLD; ++f) pr[n][i][f] = __ldg(pair[n][i] + f);
+        }
+#pragma unroll
+    for (int f = 0; f < 128 / FOLD; ++f) {
+        float c[NT][4] = {};
+#pragma unroll
+        for (int h = f * HALVES; h < (f + 1) * HALVES; ++h)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint4 w = W.w[h >> 1];
+                const uint32_t v = h & 1 ? (j ? w.w : w.z) : (j ? w.y : w.x), v8 = v >> 8;
+                const uint32_t a[4] = {v & 0x000f000fu, v & 0x00f000f0u, v8 & 0x000f000fu, v8 & 0x00f000f0u};
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    if (n == 0 || n < nt) Ops<__half>::mma(c[n], a, j ? b[n][h].z : b[n][h].x, j ? b[n][h].w : b[n][h].y);
+            }
+        const float2 s = scale_pair(W.s[f], f16);
+        const float z0 = ZERO ? float(W.z[ZERO ? f : 0] & 0xffu) : 8.f, z1 = ZERO ? float(W.z[ZERO ? f : 0] >> 8) : 8.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            if (n == 0 || n < nt) {
+                const float2 p = pr[n][0][f], q = pr[n][1][f];
+                acc[n][0] = fmaf(s.x * p.x, fmaf(0x1p24f, c[n][0], -z0 * p.y), acc[n][0]);
+                acc[n][1] = fmaf(s.x * q.x, fmaf(0x1p24f, c[n][1], -z0 * q.y), acc[n][1]);
+                acc[n][2] = fmaf(s.y * p.x, fmaf(0x1p20f, c[n][2], -z1 * p.y), acc[n][2]);
+                acc[n][3] = fmaf(s.y * q.x, fmaf(0x1p20f, c[n][3], -z1 * q.y), acc[n][3]);
+            }
+    }
+}
+
+// Adds a unit of one row tile to acc, for activations that are the sum of two bf16 numbers (hi and lo, places as x above), with plain
+// loads: they may have been written by other blocks of the same kernel.
+template <int NT, int FOLD, bool ZERO>
+__device__ __forceinline__ void unit_two(float (&acc)[NT][4], const Unit<FOLD, ZERO>& W, const __nv_bfloat16* const (&hi)[NT], const __nv_bfloat16* const (&lo)[NT], int nt, bool f16,
+                                         const Consts& k) {
+    typedef Ops<__nv_bfloat16> O;
+    constexpr int HALVES = FOLD / 32;
+#pragma unroll
+    for (int f = 0; f < 128 / FOLD; ++f) {
+        float c[NT][4] = {};
+        const uint32_t z = ZERO ? W.z[ZERO ? f : 0] : 0x0808u;
+        const uint32_t z0 = O::base0 + 0x00010001u * (z & 0xffu), z1 = O::base1 + 0x00010001u * (z >> 8);
+#pragma unroll
+        for (int h = f * HALVES; h < (f + 1) * HALVES; ++h) {
+            uint4 b[NT], d[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                if (n == 0 || n < nt) { b[n] = *reinterpret_cast<const uint4*>(hi[n] + 32 * h); d[n] = *reinterpret_cast<const uint4*>(lo[n] + 32 * h); }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint4 w = W.w[h >> 1];
+                const uint32_t u = h & 1 ? (j ? w.w : w.z) : (j ? w.y : w.x), u8 = u >> 8;
+                const uint32_t a[4] = {O::sub(O::and_or(u, k.m, k.k0), z0), O::sub(O::high(u, k.m4, k.m, k.k1), z1),
+                                       O::sub(O::and_or(u8, k.m, k.k0), z0), O::sub(O::high(u8, k.m4, k.m, k.k1), z1)};
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    if (n == 0 || n < nt) {
+                        O::mma(c[n], a, j ? d[n].z : d[n].x, j ? d[n].w : d[n].y);
+                        O::mma(c[n], a, j ? b[n].z : b[n].x, j ? b[n].w : b[n].y);
+                    }
+            }
+        }
+        const float2 s = scale_pair(W.s[f], f16);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            if (n == 0 || n < nt) {
+                acc[n][0] = fmaf(s.x, c[n][0], acc[n][0]); acc[n][1] = fmaf(s.x, c[n][1], acc[n][1]);
+                acc[n][2] = fmaf(s.y, c[n][2], acc[n][2]); acc[n][3] = fmaf(s.y, c[n][3], acc[n][3]);
             }
     }
 }
