@@ -1,18 +1,19 @@
 // Products of a few rows with 4-bit weights: Y[m, n] = sum_k X[m, k] (code - zero) scale + bias + residual.
 //
 // The weights are read once and bound the call, so what counts is to keep enough of them in flight and to spend few
-// instructions on each.  The grid is one wave of 8-warp blocks that stay for the whole call.  Row group (R row tiles) i + j * grid is the j-th of
+// instructions on each.  The grid is one wave of 16-warp blocks that stay for the whole call.  Row group (R row tiles) i + j * grid is the j-th of
 // block i, so every SM gets about the same number; 2^ksl warps share out a group's units of 128 columns (unit u goes to warp
 // u mod 2^ksl) and add their sums in shared memory in the order of the warps.  Each warp loads one unit ahead; the many warps of an SM
 // keep the rest in flight.  Activations are read through the L1 cache, which the weights pass by.
 #include "host_util.h"
 #include "w4.cuh"
 #include <algorithm>
+#include <climits>
 
 namespace vela {
 namespace {
 
-constexpr int WARPS = 8;
+constexpr int WARPS = 16;
 
 struct GemvArgs {
     w4::Weights W;
@@ -115,7 +116,7 @@ template <int XT, int NT, int R, int BLOCKS, int FOLD, bool ZERO> __global__ voi
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) red[warp][8 * n + 2 * t + (i & 1)][16 * r + g + 8 * (i >> 1)] = acc[r][n][i];
-            group_sync(1 + sl, ks * 32);
+            group_sync(sl, ks * 32);
             const int rows = min(NT * 8, a.M - m0);
             for (int i = part * 32 + lane; i < rows * (R * 16); i += ks * 32) {
                 const int c = i % (R * 16), mm = i / (R * 16);
@@ -123,7 +124,7 @@ template <int XT, int NT, int R, int BLOCKS, int FOLD, bool ZERO> __global__ voi
                 for (int w = 0; w < ks; ++w) v += red[sl * ks + w][mm][c];
                 if (rg * R * 16 + c < a.W.N) write_y<XT>(a, m0 + mm, rg * R * 16 + c, v);
             }
-            group_sync(1 + sl, ks * 32);
+            group_sync(sl, ks * 32);
         }
     }
 }
@@ -134,10 +135,13 @@ template <int XT, int NT, int R, int BLOCKS, int FOLD, bool ZERO> void launch(cu
     VELA_REQUIRE(mb <= 65535, "gemv_w4: too many rows");
     const int wave = std::max(1, sm_count() * blocks_per_sm(reinterpret_cast<const void*>(kernel), WARPS * 32, 0) / mb);
     const dim3 grid(std::min(nrg, wave), mb);
-    // as many warps on a row group as the block has left over, each with a unit at least
+    // the split with the least time: a round costs its longest warp's units and about two more to begin and to meet
     const int per = ceil_div(nrg, int(grid.x));
     a.ksl = 0;
-    while (a.ksl < 3 && (per << (a.ksl + 1)) <= WARPS && nu >= (1 << (a.ksl + 1))) ++a.ksl;
+    for (int l = 0, best = INT_MAX; (1 << l) <= WARPS && (1 << l) <= nu; ++l) {
+        const int cost = ceil_div(per << l, WARPS) * (ceil_div(nu, 1 << l) + 2);
+        if (cost < best) { best = cost; a.ksl = l; }
+    }
     kernel<<<grid, WARPS * 32, 0, st>>>(a);
 }
 template <int XT, int NT, int R, int BLOCKS> void launch(cudaStream_t st, const GemvArgs& a) {
@@ -153,10 +157,10 @@ template <int XT, int NT, int R, int BLOCKS> void launch(cudaStream_t st, const 
     }
 }
 template <int XT> void launch(cudaStream_t st, const GemvArgs& a) {
-    if (a.M <= 8) launch<XT, 1, 1, 4>(st, a);
-    else if (a.M <= 16) launch<XT, 2, 2, 2>(st, a);
-    else if (a.M <= 24) launch<XT, 3, 1, 2>(st, a);
-    else launch<XT, 4, 1, 2>(st, a);
+    if (a.M <= 8) launch<XT, 1, 1, 2>(st, a);
+    else if (a.M <= 16) launch<XT, 2, 2, 1>(st, a);
+    else if (a.M <= 24) launch<XT, 3, 1, 1>(st, a);
+    else launch<XT, 4, 1, 1>(st, a);
 }
 
 void gemv_w4(cudaStream_t st, int xtype, GemvArgs a, int xgroup) {

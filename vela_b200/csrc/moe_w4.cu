@@ -1,19 +1,17 @@
 // A mixture-of-experts layer for a few tokens on 4-bit weights, in two kernels.
 //
 // route_kernel: a cluster of 8 blocks for each token scores the experts (a warp for each), chooses, and stages the token's row for the
-// products (w4.cuh).  It also clears what the second kernel counts in.
+// products (w4_stream.cuh).  It also clears the second kernel's counters.
 //
-// expert_kernel: one wave of blocks (a cooperative launch) does the gate and up products of all chosen experts, meets at a barrier over
-// the whole grid, and does the down products.  The tokens of an expert are columns of one product, so its weights are read once for
-// every 8 NT of them.  What bounds it is the reading of the chosen experts' weights; the barrier costs about a microsecond, over which
-// the first down weights are already under way.
-//   Up: an item is one row tile of one expert (8 gate rows and their 8 up rows, so a lane holds both parts of a hidden value); ks
-//   warps share its columns.
-//   Down: an item is one row tile of the output; its sum runs over all experts' hidden columns, shared out among the block's 16 warps, or
-//   those of `split` blocks where there are few row tiles.  Sums are added in a fixed order: the last block to finish a row tile adds the parts.
+// expert_kernel: one block on each SM (a cooperative launch) does all chosen experts' gate and up products, then their down products, then the weighed sums, with
+// a barrier over the whole grid in between.  An item is one row tile of one expert, for all tokens that chose it (columns of one product, so weights are read
+// once for every 8 NT of them); a block takes a run of neighbouring items, so an expert's activations stay in its registers.  What bounds it is the reading of the
+// chosen experts' weights; a barrier costs about 1.5 us, over which the next weights are already on their way to the L2 cache.
+//   Up: a row tile is 8 gate rows and their 8 up rows, so one thread sums both parts of a hidden value, which is kept as a float.
+//   Down: the result of each token and expert by itself, as floats; then each output is summed over the token's experts in the order of their places.
 #include "host_util.h"
 #include "tc.cuh"
-#include "w4.cuh"
+#include "w4_stream.cuh"
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -26,8 +24,8 @@ namespace cg = cooperative_groups;
 constexpr int E_MAX = 1024, K_MAX = 32;
 constexpr int T_BLOCK = 32;               // tokens of one expert_kernel launch
 constexpr int RANKS = 8, ROUTE_WARPS = 8; // of route_kernel
-constexpr int WARPS = 16, BLOCKS = 1;     // of expert_kernel
-constexpr int SPLIT_MAX = 4;
+constexpr int WARPS = w4::WARPS;          // of expert_kernel
+constexpr int COUNTERS = 2;               // one for each barrier
 static __device__ unsigned g_moe_err;
 
 struct MoeArgs {
@@ -35,35 +33,47 @@ struct MoeArgs {
     const void* X; const void* router; const float* bias; void* Y;
     int32_t* ids; float* weights;     // [T][topk], the caller's or the workspace's
     __half* xs; float2* xp;           // staged rows [T][units of D], their pairs
-    __nv_bfloat16* hi; __nv_bfloat16* lo;     // hidden values [T * topk][units of I]
-    float* parts;                     // [SPLIT_MAX][row tiles of D][tokens][16]
-    unsigned* count;                  // [launch][1 + row tiles of D]: the grid barrier's, the row tiles'
+    float* h; float* o;               // hidden values [T_BLOCK * topk][I], experts' results [T_BLOCK * topk][D rounded up to 16]
+    unsigned* count;                  // [launch][COUNTERS]
     int D, I, E, topk, T, ldx, ldy, score, renorm, ytype;
     float scale;
     bool vecx, vecr;
     int t0, tn;                       // expert_kernel: its tokens
+    int room, room_bytes;             // its shared memory for sums: columns times rounds
     unsigned* err; long long limit; unsigned extra;
 };
 
-// sum of 8 products for every lane's 8 columns, W rows of the router at a time
+// a token's row times a router row, by one warp, with 8 loads of each in flight
 template <class X, class RW> __device__ __forceinline__ float dot_row(const X* x, const RW* w, int D, bool vecx, bool vecr, int lane) {
     float s[4] = {};
-    int k = 8 * lane;
-    for (; vecx && vecr && k + 3 * 256 < D; k += 4 * 256) {        // D % 8 == 0
-        float a[4][8], b[4][8];
+    if (vecx && vecr) {                               // D % 8 == 0
+        for (int k0 = 8 * lane; k0 < D; k0 += 8 * 256) {
+            uint4 a[8][sizeof(X) / 2], b[8][sizeof(RW) / 2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { load8(w + k + 256 * j, 8, true, b[j]); load8(x + k + 256 * j, 8, true, a[j]); }
+            for (int j = 0; j < 8; ++j) {
+                const int k = min(k0 + 256 * j, D - 8);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+                for (int i = 0; i < int(sizeof(RW) / 2); ++i) b[j][i] = __ldg(reinterpret_cast<const uint4*>(w + k) + i);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[j] = fmaf(a[j][i], b[j][i], s[j]);
-    }
-    for (; k < D; k += 256) {
-        float a[8], b[8];
-        load8(x + k, min(8, D - k), vecx, a);
-        load8(w + k, min(8, D - k), vecr, b);
+                for (int i = 0; i < int(sizeof(X) / 2); ++i) a[j][i] = __ldg(reinterpret_cast<const uint4*>(x + k) + i);
+            }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[0] = fmaf(a[i], b[i], s[0]);
+            for (int j = 0; j < 8; ++j) {
+                if (k0 + 256 * j >= D) break;
+                const X* u = reinterpret_cast<const X*>(a[j]);
+                const RW* v = reinterpret_cast<const RW*>(b[j]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[j & 3] = fmaf(Elem<X>::get(u[i]), Elem<RW>::get(v[i]), s[j & 3]);
+            }
+        }
+    } else {
+        for (int k = 8 * lane; k < D; k += 256) {
+            float a[8], b[8];
+            load8(w + k, min(8, D - k), vecr, b);
+            load8(x + k, min(8, D - k), vecx, a);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[0] = fmaf(a[i], b[i], s[0]);
+        }
     }
     float v = (s[0] + s[1]) + (s[2] + s[3]);
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -77,8 +87,9 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 }
 
 template <class X, class RW, int FOLD> __global__ void __cluster_dims__(RANKS, 1, 1) __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const MoeArgs a) {
-    __shared__ float p[E_MAX];
-    __shared__ uint32_t key[E_MAX];
+    __shared__ float p[E_MAX], prob[E_MAX], top[K_MAX];
+    __shared__ __align__(16) uint32_t key[E_MAX];
+    const int E4 = (a.E + 3) & ~3;
     cg::cluster_group cluster = cg::this_cluster();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tok = blockIdx.y, rank = blockIdx.x;
     const int gw = rank * ROUTE_WARPS + warp;
@@ -89,336 +100,176 @@ template <class X, class RW, int FOLD> __global__ void __cluster_dims__(RANKS, 1
         if (lane == 0) lead[e] = s;
     }
     cluster.sync();
-    if (rank != 0 || warp != 0) {
-        // all but the choosing warp: the staged row, the hidden rows' padding, the counters
-        const int i = gw - 1, n = RANKS * ROUTE_WARPS - 1, nu = w4::units(a.up);
+    if (rank != 0) {
+        // the others: the staged row, the hidden rows' padding, the counters
+        const int i = gw - ROUTE_WARPS, n = (RANKS - 1) * ROUTE_WARPS, nu = w4::units(a.up);
         for (int u = i; u < nu; u += n)
             w4::stage_unit<X, FOLD>(x + u * 128 + 4 * lane, a.D - u * 128 - 4 * lane, a.xs + (size_t(tok) * nu + u) * 128, a.xp + (size_t(tok) * nu + u) * (128 / FOLD), lane);
-        const int wide = w4::units(a.down) * 128;
-        for (int c = i * 32 + lane; c < a.topk * (wide - a.I); c += n * 32) {
-            const size_t at = (size_t(tok) * a.topk + c / (wide - a.I)) * wide + a.I + c % (wide - a.I);
-            a.hi[at] = __nv_bfloat16(0.f); a.lo[at] = __nv_bfloat16(0.f);
-        }
-        if (tok % T_BLOCK == 0) {
-            const int per = 1 + w4::row_tiles(a.down);
-            for (int c = i * 32 + lane; c < per; c += n * 32) a.count[tok / T_BLOCK * per + c] = 0;
-        }
+        if (tok % T_BLOCK == 0 && i == 0 && lane < COUNTERS) a.count[tok / T_BLOCK * COUNTERS + lane] = 0;
         return;
     }
+    // Every warp forms the softmax's maximum and sum for itself, in the same order.
+    float m = -INFINITY, sum = 0.f;
     if (a.score == 0) {
-        float m = -INFINITY, s = 0.f;
         for (int e = lane; e < a.E; e += 32) m = fmaxf(m, p[e]);
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        for (int e = lane; e < a.E; e += 32) s += p[e] = expf(p[e] - m);
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        for (int e = lane; e < a.E; e += 32) p[e] /= s;
-    } else {
-        for (int e = lane; e < a.E; e += 32) p[e] = 1.f / (1.f + expf(-p[e]));
+        for (int e = lane; e < a.E; e += 32) sum += expf(p[e] - m);
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
-    for (int e = lane; e < a.E; e += 32) {
-        const float v = p[e] + (a.bias ? a.bias[e] : 0.f);
-        key[e] = ordered(v != v ? -INFINITY : v);         // above 0, which marks an expert that was taken
+    for (int e = threadIdx.x; e < E4; e += ROUTE_WARPS * 32) {
+        uint32_t v = 0;                                    // below every expert's
+        if (e < a.E) {
+            const float q = a.score == 0 ? expf(p[e] - m) / sum : 1.f / (1.f + expf(-p[e]));
+            const float w = q + (a.bias ? a.bias[e] : 0.f);
+            prob[e] = q;
+            v = ordered(w != w ? -INFINITY : w);
+        }
+        key[e] = v;
     }
-    float mine = 0.f, sum = 0.f;
-    int id = 0;
-    for (int j = 0; j < a.topk; ++j) {
-        uint32_t best = 0;
-        int at = INT_MAX;
-        for (int e = lane; e < a.E; e += 32) if (key[e] > best) { best = key[e]; at = e; }     // the lowest of a lane's largest
-        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-        at = __reduce_min_sync(0xffffffffu, best == top ? at : INT_MAX);
-        if (at % 32 == lane) key[at] = 0;
-        __syncwarp();
-        const float w = p[at];
-        sum += w;
-        if (lane == j) { id = at; mine = w; }
+    __syncthreads();
+    // An expert's place is the number of those before it: larger ones, and equal ones of lower number.
+    for (int e = threadIdx.x; e < a.E; e += ROUTE_WARPS * 32) {
+        const uint32_t v = key[e];
+        int r = 0;
+        for (int o = 0; o < E4; o += 4) {
+            const uint4 k = *reinterpret_cast<const uint4*>(key + o);
+            r += (k.x > v || (k.x == v && o < e)) + (k.y > v || (k.y == v && o + 1 < e)) + (k.z > v || (k.z == v && o + 2 < e)) + (k.w > v || (k.w == v && o + 3 < e));
+        }
+        if (r < a.topk) { top[r] = prob[e]; a.ids[size_t(tok) * a.topk + r] = e; }
     }
-    if (lane < a.topk) {
-        a.ids[size_t(tok) * a.topk + lane] = id;
-        a.weights[size_t(tok) * a.topk + lane] = (a.renorm ? mine / sum : mine) * a.scale;
+    __syncthreads();
+    if (int(threadIdx.x) < a.topk) {
+        float s = 0.f;
+        for (int j = 0; j < a.topk; ++j) s += top[j];
+        a.weights[size_t(tok) * a.topk + threadIdx.x] = (a.renorm ? top[threadIdx.x] / s : top[threadIdx.x]) * a.scale;
     }
 }
 
-// The experts that the tokens chose: slot v has expert `expert[v]` and pairs (token * topk + place) list[first[v]] .. list[first[v + 1]), at most `most` of them.
-struct Slots {
-    int32_t* expert; int32_t* first; int32_t* list; int n;
-};
-
-// Shares of `items` items of `nu` units for one of `grid` blocks of WARPS warps: log2 of the warps on an item, so that the rounds take the least
-// time.  A round costs its longest warp's units and about two more for meeting.
-__device__ __forceinline__ int pick_ksl(int items, int nu, int grid) {
-    const int per = (items + grid - 1) / grid;
-    int best = 0, cost = INT_MAX;
-    for (int l = 0; (1 << l) <= WARPS && (1 << l) <= nu; ++l) {
-        const int c = (((per << l) + WARPS - 1) / WARPS) * (((nu + (1 << l) - 1) >> l) + 2);
-        if (c < cost) { cost = c; best = l; }
+// Waits until all blocks of the grid have come here; false (and the error word set) if they have not within the limit.
+__device__ __forceinline__ bool grid_barrier(unsigned* count, unsigned want, unsigned* err, long long limit, int* flag) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        *flag = 1;
+        __threadfence();
+        atomicAdd(count, 1u);
+        const long long t0 = clock64();
+        while (*reinterpret_cast<volatile unsigned*>(count) < want)
+            if (clock64() - t0 > limit) { atomicCAS(err, 0u, unsigned(DEVERR_TIMEOUT_OTHER)); *flag = 0; break; }
+        __threadfence();
     }
-    return best;
+    __syncthreads();
+    return *flag != 0;
 }
 
-template <int NT, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS * 32, BLOCKS) expert_kernel(const MoeArgs a) {
-    typedef w4::Unit<FOLD, ZERO> Unit;
+template <int NT, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS * 32, 1) expert_kernel(const MoeArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int s_n, s_flag;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int grid = gridDim.x, P = a.tn * a.topk, p0 = a.t0 * a.topk;
-    // shared memory: sums [WARPS][max(8 NT, tokens)][17], then the slots
-    const int rows = max(8 * NT, a.tn);
-    float* red = reinterpret_cast<float*>(smem);
-    int32_t* s_list = reinterpret_cast<int32_t*>(red + WARPS * rows * 17);
+    float* sums = reinterpret_cast<float*>(smem);
+    int32_t* s_list = reinterpret_cast<int32_t*>(smem + a.room_bytes);
     int32_t* s_ids = s_list + P;
-    int32_t* s_expert = s_ids + P;
+    int32_t* s_expert = s_ids + P;                  // slot v has expert s_expert[v] and the pairs (token * topk + place) s_at[s_first[v]] .. s_at[s_first[v + 1] - 1], 8 NT at most
     int32_t* s_first = s_expert + P;
     int32_t* s_cnt = s_first + P + 1;
-    float* s_w = reinterpret_cast<float*>(s_cnt + a.E);
-
-    for (int e = threadIdx.x; e < a.E; e += WARPS * 32) s_cnt[e] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < P; i += WARPS * 32) {
-        const int e = a.ids[p0 + i];
-        s_ids[i] = e;
-        s_w[i] = a.weights[p0 + i];
-        atomicAdd(s_cnt + e, 1);
-    }
-    __syncthreads();
-    if (warp == 0) {                                // first places and slots, by expert; s_cnt becomes the first place
-        int n = 0, at = 0;
+    int32_t* s_at = s_cnt + a.E;
+    if (warp == 0) {
+        for (int e = lane; e < a.E; e += 32) s_cnt[e] = 0;
+        __syncwarp();
+        for (int i0 = 0; i0 < P; i0 += 32) {           // each pair's place among its expert's, in the order of the pairs
+            const int i = i0 + lane, e = i < P ? a.ids[p0 + i] : -1 - lane;
+            const unsigned same = __match_any_sync(0xffffffffu, e);
+            const int before = __popc(same & ((1u << lane) - 1));
+            if (i < P) { s_ids[i] = e; s_list[i] = s_cnt[e] + before; }
+            __syncwarp();
+            if (i < P && before == 0) s_cnt[e] += __popc(same);
+            __syncwarp();
+        }
+        int n = 0, at = 0;                              // first places and slots, by expert; s_cnt becomes the first place
         for (int e0 = 0; e0 < a.E; e0 += 32) {
             const int e = e0 + lane, c = e < a.E ? s_cnt[e] : 0, v = (c + 8 * NT - 1) / (8 * NT);
+            if (__ballot_sync(0xffffffffu, c) == 0) continue;
             int ci = c, vi = v;
             for (int o = 1; o < 32; o <<= 1) {
                 const int x = __shfl_up_sync(0xffffffffu, ci, o), y = __shfl_up_sync(0xffffffffu, vi, o);
                 if (lane >= o) { ci += x; vi += y; }
             }
             for (int i = 0; i < v; ++i) { s_expert[n + vi - v + i] = e; s_first[n + vi - v + i] = at + ci - c + i * 8 * NT; }
-            if (e < a.E) s_cnt[e] = at + ci - c;
+            if (c) s_cnt[e] = at + ci - c;
             n += __shfl_sync(0xffffffffu, vi, 31);
             at += __shfl_sync(0xffffffffu, ci, 31);
         }
         if (lane == 0) { s_n = n; s_first[n] = at; }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < P; i += WARPS * 32) {
-        const int e = s_ids[i];
-        int r = 0;
-        for (int q = 0; q < i; ++q) r += s_ids[q] == e;
-        s_list[s_cnt[e] + r] = i;
+        __syncwarp();
+        for (int i0 = 0; i0 < P; i0 += 32) { const int i = i0 + lane; if (i < P) s_at[s_cnt[s_ids[i]] + s_list[i]] = i; }
     }
     __syncthreads();
     const int V = s_n;
-
-    // ------------------------------------------------ gate and up
-    {
-        const int rt_up = w4::row_tiles(a.up), nu = w4::units(a.up), items = V * rt_up, whole = a.D >> 7;
-        const int ksl = pick_ksl(items, nu, grid), ks = 1 << ksl, part = warp & (ks - 1), sl = warp >> ksl, slots = WARPS >> ksl;
-        const int wide = w4::units(a.down) * 128;
-        int it = blockIdx.x + grid * sl;
-        w4::RowPtr at;
-        auto seek = [&](int i) { const int v = i / rt_up; at = w4::row_ptr(a.up, size_t(s_expert[v]) * rt_up + (i - v * rt_up), part, lane); };
-        auto fetch = [&](Unit& s, int u) {
-            if (u < whole) w4::load_unit(s, at, a.up);
-            else w4::load_last(s, at, a.up, u);
-            w4::advance(at, a.up, ks);
-        };
-        Unit one, two;
-        if (it < items) { seek(it); fetch(one, part); }
-        for (int base = blockIdx.x; base < items; base += grid * slots, it += grid * slots) {
-            float acc[NT][4] = {};
-            int v = 0, c = 0;
-            if (it < items) {
-                v = it / rt_up;
-                c = s_first[v + 1] - s_first[v];
-                const int nt = (c + 7) >> 3;
-                const __half* x[NT];
-                const float2* pair[NT][2];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    auto tok = [&](int col) { return size_t(a.t0 + s_list[s_first[v] + min(col, c - 1)] / a.topk); };
-                    x[n] = a.xs + (tok(8 * n + g) * nu + part) * 128 + 8 * t;
-                    pair[n][0] = a.xp + (tok(8 * n + 2 * t) * nu + part) * (128 / FOLD);
-                    pair[n][1] = a.xp + (tok(8 * n + 2 * t + 1) * nu + part) * (128 / FOLD);
-                }
-                int u = part;
-                auto step = [&](const Unit& cur, Unit& nxt) {
-                    if (u + ks < nu) fetch(nxt, u + ks);
-                    w4::unit_staged<NT, FOLD, ZERO>(acc, cur, x, pair, nt, a.up.f16);
-                    u += ks;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) { x[n] += ks * 128; pair[n][0] += ks * (128 / FOLD); pair[n][1] += ks * (128 / FOLD); }
-                };
-                while (true) {
-                    step(one, two);
-                    if (u >= nu) break;
-                    step(two, one);
-                    if (u >= nu) break;
-                }
-                if (it + grid * slots < items) { seek(it + grid * slots); fetch(one, part); }
-            }
-            auto put = [&](int col, int i, float gate, float up) {       // hidden value i of column col
-                const float h = gate / (1.f + expf(-gate)) * up;
-                const __nv_bfloat16 hi = __float2bfloat16_rn(h);
-                const float hf = __bfloat162float(hi);
-                const size_t at = size_t(p0 + s_list[s_first[v] + col]) * wide + (it - v * rt_up) * 8 + i;
-                a.hi[at] = hi;
-                a.lo[at] = __float2bfloat16_rn(isinf(hf) ? 0.f : h - hf);
-            };
-            if (ks == 1) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) { const int col = 8 * n + 2 * t + i; if (col < c) put(col, g, acc[n][i], acc[n][i + 2]); }
-            } else {
-                if (it < items)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) red[(warp * rows + 8 * n + 2 * t + (i & 1)) * 17 + g + 8 * (i >> 1)] = acc[n][i];
-                __syncthreads();
-                if (it < items)
-                    for (int q = part * 32 + lane; q < c * 8; q += ks * 32) {
-                        float gate = 0.f, up = 0.f;
-                        for (int w = 0; w < ks; ++w) {
-                            const float* r = red + ((sl * ks + w) * rows + (q >> 3)) * 17;
-                            gate += r[q & 7]; up += r[8 + (q & 7)];
-                        }
-                        put(q >> 3, q & 7, gate, up);
-                    }
-                __syncthreads();
-            }
+    // Runs of items: this block's row tiles of one slot after another.  ask: a run's weights on their way to the L2 cache, 64 KB of them at most
+    auto ask = [&](const w4::Weights& W, int it, int hi) {
+        if (threadIdx.x == 0 && it < hi) {
+            const int rt = w4::row_tiles(W), v = it / rt, n = min(min(hi - it, rt - (it - v * rt)), max(1, 65536 / (W.kt * 512)));
+            w4::prefetch_l2(W.q + (size_t(s_expert[v]) * rt + (it - v * rt)) * W.kt * 32, min(n * W.kt * 512, 65536));
         }
-    }
-
-    // ------------------------------------------------ down: what is fetched first does not depend on the hidden values
-    const int rt_down = w4::row_tiles(a.down), nu = w4::units(a.down), total = V * nu, whole = a.I >> 7;
-    int split = 1;
-    while (split < SPLIT_MAX && rt_down * split * 2 <= grid && total >= split * 2 * WARPS) split *= 2;
-    const int items = rt_down * split;
-    const w4::Consts k = w4::consts<__nv_bfloat16>();
-    Unit one, two;
-    w4::RowPtr at;
-    auto span = [&](int s, int w) { return int((long long)total * (s * WARPS + w) / (split * WARPS)); };
-    auto fetch = [&](Unit& s, int rt, int q, bool seek) {
-        const int v = q / nu, u = q - v * nu;
-        if (seek || u == 0) at = w4::row_ptr(a.down, size_t(s_expert[v]) * rt_down + rt, u, lane);
-        if (u < whole) w4::load_unit(s, at, a.down);
-        else w4::load_last(s, at, a.down, u);
-        w4::advance(at, a.down, 1);
     };
-    {
-        const int s = blockIdx.x / rt_down, q = span(s, warp);
-        if (int(blockIdx.x) < items && q < span(s, warp + 1)) fetch(one, blockIdx.x - s * rt_down, q, true);
-    }
+    auto runs = [&](const w4::Weights& W, auto run) {
+        const int rt = w4::row_tiles(W);
+        const int lo = int((long long)V * rt * blockIdx.x / grid), hi = int((long long)V * rt * (blockIdx.x + 1) / grid);
+        for (int it = lo; it < hi;) {
+            const int v = it / rt, r0 = it - v * rt, n = min(rt - r0, hi - it);
+            it += n;
+            ask(W, it, hi);
+            run(v, size_t(s_expert[v]) * rt, r0, r0 + n, s_first[v + 1] - s_first[v]);
+        }
+    };
+    auto pair_of = [&](int v, int col) { return s_at[s_first[v] + col]; };
 
-    // ------------------------------------------------ all hidden values are written
-    unsigned* count = a.count + a.t0 / T_BLOCK * (1 + rt_down);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        atomicAdd(count, 1u);
-        s_flag = 0;
-        const long long t0 = clock64();
-        volatile unsigned* c = count;
-        while (*c < grid + a.extra)
-            if (clock64() - t0 > a.limit) { atomicCAS(a.err, 0u, unsigned(DEVERR_TIMEOUT_OTHER)); s_flag = 1; break; }
-        __threadfence();
-    }
-    __syncthreads();
-    if (s_flag) return;
+    runs(a.up, [&](int v, size_t tile0, int r0, int r1, int c) {
+        const int nu = w4::units(a.up), room = a.room / c;
+        w4::stream<w4::F, NT, NT == 1 && FOLD == 128 ? 2 : 1, FOLD, ZERO, true>(a.up, tile0, r0, r1, c, sums, room,
+            [&](int n, int u, uint32_t (&b)[16], w4::Pairs<FOLD>& p) {
+                auto at = [&](int col) { return size_t(a.t0 + pair_of(v, min(8 * n + col, c - 1)) / a.topk) * nu + u; };     // any row where there is none: its column is not used
+                w4::load_staged<FOLD>(b, p, a.xs + at(g) * 128 + 8 * t, a.xp + at(2 * t) * (128 / FOLD), a.xp + at(2 * t + 1) * (128 / FOLD));
+            },
+            [&](int rt, int col, int i, float gate, float up) { a.h[size_t(pair_of(v, col)) * a.I + rt * 8 + i] = gate / (1.f + expf(-gate)) * up; });
+    });
+    unsigned* count = a.count + a.t0 / T_BLOCK * COUNTERS;
+    ask(a.down, int((long long)V * w4::row_tiles(a.down) * blockIdx.x / grid), int((long long)V * w4::row_tiles(a.down) * (blockIdx.x + 1) / grid));
+    if (!grid_barrier(count, grid + a.extra, a.err, a.limit, &s_flag)) return;
 
-    for (int it = blockIdx.x; it < items; it += grid) {
-        const int s = it / rt_down, rt = it - s * rt_down, end = span(s, warp + 1);
-        int q = span(s, warp);
-        float* mine = red + warp * rows * 17;          // [token][17]
-        for (int i = lane; i < a.tn * 17; i += 32) mine[i] = 0.f;
-        __syncwarp();
-        if (it != int(blockIdx.x) && q < end) fetch(one, rt, q, true);
-        float acc[NT][4] = {};
-        const __nv_bfloat16* hi[NT];
-        const __nv_bfloat16* lo[NT];
-        bool fresh = true;
-        auto step = [&](const Unit& cur, Unit& nxt) {
-            if (q + 1 < end) fetch(nxt, rt, q + 1, false);
-            const int v = q / nu, u = q - v * nu, c = s_first[v + 1] - s_first[v], nt = (c + 7) >> 3;
-            if (fresh) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const size_t r = (size_t(p0 + s_list[s_first[v] + min(8 * n + g, c - 1)]) * nu + u) * 128 + 8 * t;
-                    hi[n] = a.hi + r; lo[n] = a.lo + r;
-                }
-                fresh = false;
-            }
-            w4::unit_two<NT, FOLD, ZERO>(acc, cur, hi, lo, nt, a.down.f16, k);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) { hi[n] += 128; lo[n] += 128; }
-            ++q;
-            if (u + 1 < nu && q < end) return;
-            fresh = true;                              // the expert's last unit here: its tokens' sums, weighed
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int col = 8 * n + 2 * t + (i & 1);
-                    if (col < c) {
-                        const int p = s_list[s_first[v] + col];
-                        float* d = mine + (p / a.topk) * 17 + g + 8 * (i >> 1);
-                        *d = fmaf(s_w[p], acc[n][i], *d);
-                    }
-                    acc[n][i] = 0.f;
-                }
-            __syncwarp();
-        };
-        while (q < end) {
-            step(one, two);
-            if (q >= end) break;
-            step(two, one);
-        }
-        __syncthreads();
-        auto write = [&](int i, float v) {
-            const int n = rt * 16 + (i & 15);
-            if (n >= a.D) return;
-            const size_t at = size_t(a.t0 + (i >> 4)) * a.ldy + n;
-            if (a.ytype == VELA_T_BF16) static_cast<__nv_bfloat16*>(a.Y)[at] = __float2bfloat16_rn(v);
-            else static_cast<__half*>(a.Y)[at] = __float2half_rn(v);
-        };
-        const size_t part = size_t(rt_down) * a.tn * 16;
-        for (int i = threadIdx.x; i < a.tn * 16; i += WARPS * 32) {
-            float v = 0.f;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) v += red[(w * rows + (i >> 4)) * 17 + (i & 15)];
-            if (split == 1) write(i, v);
-            else a.parts[s * part + size_t(rt) * a.tn * 16 + i] = v;
-        }
-        if (split > 1) {
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) s_flag = atomicAdd(count + 1 + rt, 1u) == unsigned(split - 1);
-            __syncthreads();
-            if (s_flag) {                              // the last of the row tile's blocks
-                __threadfence();
-                for (int i = threadIdx.x; i < a.tn * 16; i += WARPS * 32) {
-                    float v = 0.f;
-                    for (int z = 0; z < split; ++z) v += __ldcg(a.parts + z * part + size_t(rt) * a.tn * 16 + i);
-                    write(i, v);
-                }
-            }
-        }
-        __syncthreads();
+    const int wide = w4::row_tiles(a.down) * 16;
+    runs(a.down, [&](int v, size_t tile0, int r0, int r1, int c) {
+        w4::stream<w4::H, NT, 1, FOLD, ZERO, false>(a.down, tile0, r0, r1, c, sums, a.room / c,
+            [&](int n, int u, uint32_t (&b)[32], w4::Pairs<FOLD>& p) {
+                w4::load_floats<FOLD>(b, p, a.h + size_t(pair_of(v, min(8 * n + g, c - 1))) * a.I + u * 128 + 8 * t, a.I - u * 128 - 8 * t, t);
+            },
+            [&](int rt, int col, int row, float y, float) { a.o[size_t(pair_of(v, col)) * wide + rt * 16 + row] = y; });
+    });
+    if (!grid_barrier(count + 1, grid + a.extra, a.err, a.limit, &s_flag)) return;
+
+    for (int i = blockIdx.x * (WARPS * 32) + threadIdx.x; i < a.tn * a.D; i += grid * (WARPS * 32)) {
+        const int tok = i / a.D, n = i - tok * a.D;
+        float y = 0.f;
+        for (int j = 0; j < a.topk; ++j)
+            y = fmaf(__ldg(a.weights + size_t(a.t0 + tok) * a.topk + j), __ldcg(a.o + size_t(tok * a.topk + j) * wide + n), y);
+        const size_t at = size_t(a.t0 + tok) * a.ldy + n;
+        if (a.ytype == VELA_T_BF16) static_cast<__nv_bfloat16*>(a.Y)[at] = __float2bfloat16_rn(y);
+        else static_cast<__half*>(a.Y)[at] = __float2half_rn(y);
     }
 }
 
-struct Layout { size_t ids, weights, xs, xp, hi, lo, parts, count, bytes; };
+struct Layout { size_t ids, weights, xs, xp, h, o, count, bytes; };
 Layout layout(const vela_moe& L, int T) {
-    Layout o;
-    const size_t n = size_t(T) * L.topk, nu = (size_t(L.D) + 127) / 128, nh = (size_t(L.I) + 127) / 128, rt = (size_t(L.D) + 15) / 16, fold = 128 / L.gate_up.group;
+    Layout w;
+    const size_t n = size_t(T) * L.topk, nu = (size_t(L.D) + 127) / 128, fold = 128 / L.gate_up.group, some = size_t(std::min(T, T_BLOCK)) * L.topk;
     size_t at = 0;
     auto take = [&](size_t b) { const size_t r = at; at += align_up(b, 256); return r; };
-    o.ids = take(n * 4); o.weights = take(n * 4);
-    o.xs = take(T * nu * 256); o.xp = take(T * nu * fold * 8);
-    o.hi = take(n * nh * 256); o.lo = take(n * nh * 256);
-    o.parts = take(SPLIT_MAX * rt * std::min(T, T_BLOCK) * 64);
-    o.count = take((size_t(T) + T_BLOCK - 1) / T_BLOCK * (1 + rt) * 4);
-    o.bytes = at;
-    return o;
+    w.ids = take(n * 4); w.weights = take(n * 4);
+    w.xs = take(T * nu * 256); w.xp = take(T * nu * fold * 8);
+    w.h = take(some * L.I * 4); w.o = take(some * ((size_t(L.D) + 15) / 16 * 16) * 4);
+    w.count = take((size_t(T) + T_BLOCK - 1) / T_BLOCK * COUNTERS * 4);
+    w.bytes = at;
+    return w;
 }
 
 void check(const vela_moe& L, int T) {
@@ -434,14 +285,15 @@ void check(const vela_moe& L, int T) {
 
 template <int NT, int FOLD, bool ZERO> void launch_experts(cudaStream_t st, MoeArgs a) {
     auto* kernel = expert_kernel<NT, FOLD, ZERO>;
-    const int rows = std::max(8 * NT, a.tn), P = a.tn * a.topk;
-    const size_t smem = size_t(WARPS) * rows * 17 * 4 + (size_t(P) * 5 + 1 + a.E) * 4;
-    constexpr size_t most = size_t(WARPS) * T_BLOCK * 17 * 4 + (size_t(T_BLOCK) * K_MAX * 5 + 1 + E_MAX) * 4;
+    // room for the sums of so many columns times rounds, then the slots
+    a.room = NT == 1 ? 96 : 48;
+    a.room_bytes = int(w4::sum_bytes(1, a.room));
+    const size_t smem = a.room_bytes + (size_t(a.tn) * a.topk * 5 + 1 + a.E) * 4;
+    constexpr size_t most = w4::sum_bytes(1, 96) + (size_t(T_BLOCK) * K_MAX * 5 + 1 + E_MAX) * 4;
     static std::atomic<int> ready[64];
     once_per_device(ready, [&] { VELA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most))); });
-    const int wave = sm_count() * blocks_per_sm(reinterpret_cast<const void*>(kernel), WARPS * 32, smem);
     void* args[] = {&a};
-    VELA_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kernel), dim3(wave), dim3(WARPS * 32), args, smem, st));
+    VELA_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kernel), dim3(sm_count()), dim3(WARPS * 32), args, smem, st));
 }
 template <int FOLD> void launch(cudaStream_t st, MoeArgs a, int router_type) {
     const dim3 grid(RANKS, a.T);
@@ -454,8 +306,10 @@ template <int FOLD> void launch(cudaStream_t st, MoeArgs a, int router_type) {
     }
     for (a.t0 = 0; a.t0 < a.T; a.t0 += T_BLOCK) {
         a.tn = std::min(T_BLOCK, a.T - a.t0);
-        if (a.up.zero) a.tn <= 8 ? launch_experts<1, FOLD, true>(st, a) : launch_experts<2, FOLD, true>(st, a);
-        else a.tn <= 8 ? launch_experts<1, FOLD, false>(st, a) : launch_experts<2, FOLD, false>(st, a);
+        // 16 columns at a time where an expert has more than 8 tokens as a rule (its weights are then read once), else 8
+        const bool one = a.tn <= 8 || a.tn * a.topk <= 6 * a.E;
+        if (a.up.zero) one ? launch_experts<1, FOLD, true>(st, a) : launch_experts<2, FOLD, true>(st, a);
+        else one ? launch_experts<1, FOLD, false>(st, a) : launch_experts<2, FOLD, false>(st, a);
     }
 }
 
@@ -480,9 +334,8 @@ void moe_w4(cudaStream_t st, int type, const void* X, int ldx, int T, const vela
     a.weights = weights ? weights : reinterpret_cast<float*>(w + o.weights);
     a.xs = reinterpret_cast<__half*>(w + o.xs);
     a.xp = reinterpret_cast<float2*>(w + o.xp);
-    a.hi = reinterpret_cast<__nv_bfloat16*>(w + o.hi);
-    a.lo = reinterpret_cast<__nv_bfloat16*>(w + o.lo);
-    a.parts = reinterpret_cast<float*>(w + o.parts);
+    a.h = reinterpret_cast<float*>(w + o.h);
+    a.o = reinterpret_cast<float*>(w + o.o);
     a.count = reinterpret_cast<unsigned*>(w + o.count);
     a.D = L.D; a.I = L.I; a.E = L.E; a.topk = L.topk; a.T = T; a.ldx = ldx; a.ldy = ldy; a.score = L.score; a.renorm = L.renorm; a.scale = L.scale;
     a.ytype = type;

@@ -281,128 +281,6 @@ __device__ __forceinline__ void unit(float (&acc)[R][NT][4], const Unit<FOLD, ZE
     }
 }
 
-// ---------------------------------------------------------------- staged activations
-// Rows of f16 values that were brought into a form in which a weight costs less, once, by whoever produces them: whole units (zeros
-// beyond K), and for each fold of a unit a pair {factor that the staged values have lost, sum of the staged values}.  The bits of a
-// nibble at the bottom of a 16-bit half are, as they stand, the (subnormal) f16 number code * 2^-24, four bits up code * 2^-20, both
-// exact and taken by the tensor cores at full rate: a word takes one shift and four masks (f16 operands as above: 9, bf16: 11), and zero times the sum
-// is taken off the sum of products.
-
-// Brings columns 4 lane .. 4 lane + 3 of a unit (n of them exist) of a row of X to `out` (the unit's 128 values), a warp together; lane 0
-// of each fold writes its pair.
-template <class X, int FOLD> __device__ __forceinline__ void stage_unit(const X* p, int n, __half* out, float2* pair, int lane) {
-    float v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? Elem<X>::get(p[i]) : 0.f;
-    float back = 1.f;
-    if constexpr (Elem<X>::code != VELA_T_F16) {
-        // The largest value is brought into [2^14, 2^15) by a power of two: bf16's 8 bits then fit f16 exactly down to 2^-31 of it, and
-        // what is smaller is rounded to 2^-39 of it, below a 32-bit sum's own rounding.
-        const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(__float_as_uint(v[0]) & 0x7fffffffu, __float_as_uint(v[1]) & 0x7fffffffu),
-                                                                max(__float_as_uint(v[2]) & 0x7fffffffu, __float_as_uint(v[3]) & 0x7fffffffu)));
-        int e = int(top >> 23) - 127;                      // 128: an infinity or a NaN, which stays one
-        e = e > 127 ? 127 : e < -100 ? -100 : e;           // both factors are normal floats
-        const float fwd = __uint_as_float(uint32_t(127 + 14 - e) << 23);
-        back = __uint_as_float(uint32_t(127 - 14 + e) << 23);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] *= fwd;
-    }
-    const __half2 lo = __floats2half2_rn(v[0], v[1]), hi = __floats2half2_rn(v[2], v[3]);
-    *reinterpret_cast<uint2*>(out + 4 * lane) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-    const float2 fl = __half22float2(lo), fh = __half22float2(hi);
-    float sum = (fl.x + fl.y) + (fh.x + fh.y);
-#pragma unroll
-    for (int o = 1; o < FOLD / 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane % (FOLD / 4) == 0) pair[lane / (FOLD / 4)] = make_float2(back, sum);
-}
-
-// Adds a unit of one row tile to acc.  x[n]: this lane's place in column tile n (row g, column 8 t of the unit); pair[n][i]: the unit's first pair of
-// activation row 2t + i; nt: the column tiles that hold any row.
-template <int NT, int FOLD, bool ZERO>
-__device__ __forceinline__ void unit_staged(float (&acc)[NT][4], const Unit<FOLD, ZERO>& W, const __half* const (&x)[NT], const float2* const (&pair)[NT][2], int nt, bool f16) {
-    constexpr int HALVES = FOLD / 32;
-    uint4 b[NT][4];
-    float2 pr[NT][2][128 / FOLD];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-        if (n == 0 || n < nt) {
-#pragma unroll
-            for (int h = 0; h < 4; ++h) b[n][h] = __ldg(reinterpret_cast<const uint4*>(x[n] + 32 * h));
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int f = 0; f < 128 / FOLD; ++f) pr[n][i][f] = __ldg(pair[n][i] + f);
-        }
-#pragma unroll
-    for (int f = 0; f < 128 / FOLD; ++f) {
-        float c[NT][4] = {};
-#pragma unroll
-        for (int h = f * HALVES; h < (f + 1) * HALVES; ++h)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint4 w = W.w[h >> 1];
-                const uint32_t v = h & 1 ? (j ? w.w : w.z) : (j ? w.y : w.x), v8 = v >> 8;
-                const uint32_t a[4] = {v & 0x000f000fu, v & 0x00f000f0u, v8 & 0x000f000fu, v8 & 0x00f000f0u};
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    if (n == 0 || n < nt) Ops<__half>::mma(c[n], a, j ? b[n][h].z : b[n][h].x, j ? b[n][h].w : b[n][h].y);
-            }
-        const float2 s = scale_pair(W.s[f], f16);
-        const float z0 = ZERO ? float(W.z[ZERO ? f : 0] & 0xffu) : 8.f, z1 = ZERO ? float(W.z[ZERO ? f : 0] >> 8) : 8.f;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            if (n == 0 || n < nt) {
-                const float2 p = pr[n][0][f], q = pr[n][1][f];
-                acc[n][0] = fmaf(s.x * p.x, fmaf(0x1p24f, c[n][0], -z0 * p.y), acc[n][0]);
-                acc[n][1] = fmaf(s.x * q.x, fmaf(0x1p24f, c[n][1], -z0 * q.y), acc[n][1]);
-                acc[n][2] = fmaf(s.y * p.x, fmaf(0x1p20f, c[n][2], -z1 * p.y), acc[n][2]);
-                acc[n][3] = fmaf(s.y * q.x, fmaf(0x1p20f, c[n][3], -z1 * q.y), acc[n][3]);
-            }
-    }
-}
-
-// Adds a unit of one row tile to acc, for activations that are the sum of two bf16 numbers (hi and lo, places as x above), with plain
-// loads: they may have been written by other blocks of the same kernel.
-template <int NT, int FOLD, bool ZERO>
-__device__ __forceinline__ void unit_two(float (&acc)[NT][4], const Unit<FOLD, ZERO>& W, const __nv_bfloat16* const (&hi)[NT], const __nv_bfloat16* const (&lo)[NT], int nt, bool f16,
-                                         const Consts& k) {
-    typedef Ops<__nv_bfloat16> O;
-    constexpr int HALVES = FOLD / 32;
-#pragma unroll
-    for (int f = 0; f < 128 / FOLD; ++f) {
-        float c[NT][4] = {};
-        const uint32_t z = ZERO ? W.z[ZERO ? f : 0] : 0x0808u;
-        const uint32_t z0 = O::base0 + 0x00010001u * (z & 0xffu), z1 = O::base1 + 0x00010001u * (z >> 8);
-#pragma unroll
-        for (int h = f * HALVES; h < (f + 1) * HALVES; ++h) {
-            uint4 b[NT], d[NT];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-                if (n == 0 || n < nt) { b[n] = *reinterpret_cast<const uint4*>(hi[n] + 32 * h); d[n] = *reinterpret_cast<const uint4*>(lo[n] + 32 * h); }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint4 w = W.w[h >> 1];
-                const uint32_t u = h & 1 ? (j ? w.w : w.z) : (j ? w.y : w.x), u8 = u >> 8;
-                const uint32_t a[4] = {O::sub(O::and_or(u, k.m, k.k0), z0), O::sub(O::high(u, k.m4, k.m, k.k1), z1),
-                                       O::sub(O::and_or(u8, k.m, k.k0), z0), O::sub(O::high(u8, k.m4, k.m, k.k1), z1)};
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    if (n == 0 || n < nt) {
-                        O::mma(c[n], a, j ? d[n].z : d[n].x, j ? d[n].w : d[n].y);
-                        O::mma(c[n], a, j ? b[n].z : b[n].x, j ? b[n].w : b[n].y);
-                    }
-            }
-        }
-        const float2 s = scale_pair(W.s[f], f16);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            if (n == 0 || n < nt) {
-                acc[n][0] = fmaf(s.x, c[n][0], acc[n][0]); acc[n][1] = fmaf(s.x, c[n][1], acc[n][1]);
-                acc[n][2] = fmaf(s.y, c[n][2], acc[n][2]); acc[n][3] = fmaf(s.y, c[n][3], acc[n][3]);
-            }
-    }
-}
-
 }  // namespace w4
 
 // checks a descriptor and brings it into the kernels' form; `name` begins the messages
