@@ -1,20 +1,23 @@
-// A mixture-of-experts layer for a few tokens on 4-bit weights, in two kernels.
+// A mixture-of-experts layer for a few tokens on 4-bit weights, in two kernels, of two forms.  What bounds the layer is the reading of the chosen experts' weights; with one or
+// two tokens it is latency.
 //
-// route_kernel: a cluster of 8 blocks for each token scores the experts (a warp for each), chooses, and stages the token's row for the
-// products (w4_stream.cuh).  It also clears the second kernel's counters.
+// Very few tokens (moe_few.cuh): few_up_kernel routes and does the gate and up products, few_down_kernel the down products and their weighed sums.
 //
-// expert_kernel: one block on each SM (a cooperative launch) does all chosen experts' gate and up products, then their down products, then the weighed sums, with
-// a barrier over the whole grid in between.  An item is one row tile of one expert, for all tokens that chose it (columns of one product, so weights are read
-// once for every 8 NT of them); a block takes a run of neighbouring items, so an expert's activations stay in its registers.  What bounds it is the reading of the
-// chosen experts' weights; a barrier costs about 1.5 us, over which the next weights are already on their way to the L2 cache.
+// Else: route_kernel, a cluster of 8 blocks for each token, scores the experts (a warp for each), chooses, and stages the token's row for the products (w4_stream.cuh); it also clears
+// the other kernel's counters.  expert_kernel, one block on each SM (a cooperative launch), does all chosen experts' gate and up products, then their down products, then the weighed
+// sums, with a barrier over the whole grid in between.  An item is one row tile of one expert, for all tokens that chose it (columns of one product, so weights are read once
+// for every 8 NT of them); a block takes a run of neighbouring items, so an expert's activations stay in its registers.  A barrier costs about 1.5 us, over which the next
+// weights are already on their way to the L2 cache.
 //   Up: a row tile is 8 gate rows and their 8 up rows, so one thread sums both parts of a hidden value, which is kept as a float.
 //   Down: the result of each token and expert by itself, as floats; then each output is summed over the token's experts in the order of their places.
 #include "host_util.h"
 #include "tc.cuh"
+#include "moe_few.cuh"
 #include "w4_stream.cuh"
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cmath>
 #include <cooperative_groups.h>
 
 namespace vela {
@@ -25,6 +28,8 @@ constexpr int E_MAX = 1024, K_MAX = 32;
 constexpr int T_BLOCK = 32;               // tokens of one expert_kernel launch
 constexpr int RANKS = 8, ROUTE_WARPS = 8; // of route_kernel
 constexpr int WARPS = w4::WARPS;          // of expert_kernel
+constexpr int FEW_SMEM = 96 * 1024;           // of two blocks on an SM
+constexpr size_t FEW_ROUTER = 512 * 1024;     // elements of the router that a cluster reads
 constexpr int COUNTERS = 2;               // one for each barrier
 static __device__ unsigned g_moe_err;
 
@@ -33,12 +38,14 @@ struct MoeArgs {
     const void* X; const void* router; const float* bias; void* Y;
     int32_t* ids; float* weights;     // [T][topk], the caller's or the workspace's
     __half* xs; float2* xp;           // staged rows [T][units of D], their pairs
+    __nv_bfloat16* hi; __nv_bfloat16* lo;     // few tokens: hidden values [T * topk][units of I]
     float* h; float* o;               // hidden values [T_BLOCK * topk][I], experts' results [T_BLOCK * topk][D rounded up to 16]
     unsigned* count;                  // [launch][COUNTERS]
     int D, I, E, topk, T, ldx, ldy, score, renorm, ytype;
     float scale;
     bool vecx, vecr;
     int t0, tn;                       // expert_kernel: its tokens
+    w4::Split split_up, split_down;
     int room, room_bytes;             // its shared memory for sums: columns times rounds
     unsigned* err; long long limit; unsigned extra;
 };
@@ -145,17 +152,172 @@ template <class X, class RW, int FOLD> __global__ void __cluster_dims__(RANKS, 1
     }
 }
 
+template <class X, int FOLD, bool ZERO> __global__ void __cluster_dims__(few::RANKS, 1, 1) __launch_bounds__(few::WARPS * 32, 2) few_up_kernel(const MoeArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float s_z[few::TOKENS][few::EXPERTS], s_p[few::TOKENS][few::EXPERTS], s_top[few::PAIRS];
+    __shared__ __align__(16) uint32_t s_key[few::TOKENS][few::EXPERTS];
+    __shared__ int32_t s_ids[few::PAIRS];
+    __shared__ float s_sum[few::WARPS][16];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, nu = w4::units(a.up), rank = blockIdx.x % few::RANKS;
+    const X* x = static_cast<const X*>(a.X);
+    __half* xs = reinterpret_cast<__half*>(smem);
+    float2* xp = reinterpret_cast<float2*>(smem + size_t(a.T) * nu * 256);
+    float* part = reinterpret_cast<float*>(smem + few::stage_bytes<FOLD>(a.T, nu));
+    const int mine = few::score_tiles(a.E) * 16;          // experts whose scores this block forms, at most
+    few::part_scores<X>(x, a.ldx, a.T, static_cast<const X*>(a.router), a.E, a.D, part + warp * mine * few::PART, rank, warp, lane);
+    for (int i = warp; i < a.T * nu; i += few::WARPS) {
+        const int tok = w4::quot(i, nu), u = i - tok * nu;
+        w4::stage_unit<X, FOLD>(x + size_t(tok) * a.ldx + u * 128 + 4 * lane, a.D - u * 128 - 4 * lane, xs + size_t(i) * 128, xp + size_t(i) * (128 / FOLD), lane);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < mine * few::TOKENS; i += few::WARPS * 32) {
+        const int at = i >> 3, tok = i & 7, e = (at / 16 * few::RANKS + rank) * 16 + at % 16;
+        if (e >= a.E || tok >= a.T) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < few::WARPS; ++w) v += part[(w * mine + at) * few::PART + tok];
+        for (int r = 0; r < few::RANKS; ++r) cluster.map_shared_rank(&s_z[0][0], r)[tok * few::EXPERTS + e] = v;
+    }
+    cluster.sync();
+    // probabilities and keys: a warp for each token
+    const int E4 = (a.E + 3) & ~3;
+    if (warp < a.T) {
+        const float* z = s_z[warp];
+        float m = -INFINITY, sum = 0.f;
+        if (a.score == 0) {
+            for (int e = lane; e < a.E; e += 32) m = fmaxf(m, z[e]);
+            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int e = lane; e < a.E; e += 32) sum += expf(z[e] - m);
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+        for (int e = lane; e < E4; e += 32) {
+            uint32_t v = 0;                                // below every expert's
+            if (e < a.E) {
+                const float q = a.score == 0 ? expf(z[e] - m) / sum : 1.f / (1.f + expf(-z[e])), w = q + (a.bias ? __ldg(a.bias + e) : 0.f);
+                s_p[warp][e] = q;
+                v = ordered(w != w ? -INFINITY : w);
+            }
+            s_key[warp][e] = v;
+        }
+    }
+    __syncthreads();
+    // an expert's place is the number of those before it: larger ones, and equal ones of lower number
+    for (int i = threadIdx.x; i < a.T * few::EXPERTS; i += few::WARPS * 32) {
+        const int tok = i / few::EXPERTS, e = i % few::EXPERTS;
+        if (e >= a.E) continue;
+        const uint32_t v = s_key[tok][e];
+        int r = 0;
+#pragma unroll 1
+        for (int o = 0; o < E4; o += 4) {
+            const uint4 k = *reinterpret_cast<const uint4*>(&s_key[tok][o]);
+            r += (k.x > v || (k.x == v && o < e)) + (k.y > v || (k.y == v && o + 1 < e)) + (k.z > v || (k.z == v && o + 2 < e)) + (k.w > v || (k.w == v && o + 3 < e));
+        }
+        if (r < a.topk) { s_ids[tok * a.topk + r] = e; s_top[tok * a.topk + r] = s_p[tok][e]; }
+    }
+    __syncthreads();
+    if (blockIdx.x == 0 && int(threadIdx.x) < a.T * a.topk) {
+        const int tok = w4::quot(threadIdx.x, a.topk);
+        float s = 0.f;
+        for (int j = 0; j < a.topk; ++j) s += s_top[tok * a.topk + j];
+        a.ids[threadIdx.x] = s_ids[threadIdx.x];
+        a.weights[threadIdx.x] = (a.renorm ? s_top[threadIdx.x] / s : s_top[threadIdx.x]) * a.scale;
+    }
+    // the hidden rows' padding
+    const int wide = w4::units(a.down) * 128, P = a.T * a.topk;
+    for (int p = blockIdx.x; p < P; p += gridDim.x)
+        for (int c = a.I + threadIdx.x; c < wide; c += few::WARPS * 32) { a.hi[size_t(p) * wide + c] = __nv_bfloat16(0.f); a.lo[size_t(p) * wide + c] = __nv_bfloat16(0.f); }
+    const int rt = w4::row_tiles(a.up), items = P * rt, ks = a.split_up.ks, slots = a.split_up.slots, sl = w4::quot(warp, ks), kw = warp - sl * ks;
+    for (int base = blockIdx.x; base < items; base += gridDim.x * slots) {
+        const int it = base + gridDim.x * sl;
+        float acc[2] = {};
+        const int p = w4::quot(min(it, items - 1), rt), r = it - p * rt;
+        if (sl < slots && it < items) {
+            const size_t tile = size_t(s_ids[p]) * rt + r;
+            const __half* row = xs + size_t(w4::quot(p, a.topk)) * nu * 128 + 8 * t;
+            const float2* pair = xp + size_t(w4::quot(p, a.topk)) * nu * (128 / FOLD);
+            constexpr int U = 2;                           // units under way at a time
+            w4::RowPtr at = w4::row_ptr(a.up, tile, kw, lane);
+            if (kw == 0 && lane == 0) w4::prefetch_l2(at.q, a.up.kt * 512);
+#pragma unroll 1
+            for (int u = kw; u < nu; u += U * ks) {
+                w4::Unit<FOLD, ZERO> w[U];
+#pragma unroll
+                for (int i = 0; i < U; ++i)
+                    if (u + i * ks < nu) { w4::load_last(w[i], at, a.up, u + i * ks); w4::advance(at, a.up, ks); }
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const int v = u + i * ks;
+                    if (v < nu) few::one_staged<FOLD, ZERO>(acc, w[i], row + v * 128, pair + v * (128 / FOLD), a.up.f16);
+                }
+            }
+        }
+        if (t == 0) { s_sum[warp][lane >> 2] = acc[0]; s_sum[warp][8 + (lane >> 2)] = acc[1]; }
+        __syncthreads();
+        if (kw == 0 && sl < slots && lane < 8 && it < items) {
+            float gate = 0.f, up = 0.f;
+            for (int w = 0; w < ks; ++w) { gate += s_sum[warp + w][lane]; up += s_sum[warp + w][8 + lane]; }
+            const float h = gate / (1.f + expf(-gate)) * up;
+            const __nv_bfloat16 hi = __float2bfloat16_rn(h);
+            const float hf = __bfloat162float(hi);
+            const size_t at = size_t(p) * wide + r * 8 + lane;
+            a.hi[at] = hi;
+            a.lo[at] = __float2bfloat16_rn(isinf(hf) ? 0.f : h - hf);
+        }
+        __syncthreads();
+    }
+}
+
+template <int FOLD, bool ZERO> __global__ void __launch_bounds__(few::WARPS * 32, 2) few_down_kernel(const MoeArgs a) {
+    __shared__ float s_sum[few::WARPS][16];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int rt = w4::row_tiles(a.down), nu = w4::units(a.down), items = a.T * rt, n = a.topk * nu, wide = nu * 128;
+    const w4::Consts k = w4::consts<__nv_bfloat16>();
+    // the two terms of a hidden value are columns 0 and 1 of the product (and 2 to 7 again, which are not used)
+    const __nv_bfloat16* h = (g & 1 ? a.lo : a.hi) + 8 * t;
+    for (int it = blockIdx.x; it < items; it += gridDim.x) {
+        const int tok = w4::quot(it, rt), r = it - tok * rt;
+        float acc[2] = {};
+#pragma unroll 1
+        for (int q = warp; q < n; q += few::WARPS) {
+            const int j = w4::quot(q, nu), u = q - j * nu, p = tok * a.topk + j;
+            w4::Unit<FOLD, ZERO> w[1];
+            w4::load_last(w[0], w4::row_ptr(a.down, size_t(__ldg(a.ids + p)) * rt + r, u, lane), a.down, u);
+            float c[1][1][4] = {};
+            const __nv_bfloat16* x[1] = {h + size_t(p) * wide + u * 128};
+            w4::unit<VELA_T_BF16, true, 1, 1>(c, w, x, 0, a.down.f16, k, [](int, int) { return make_float2(1.f, 1.f); });
+            const float y = __ldg(a.weights + p);
+            acc[0] = fmaf(y, c[0][0][0] + c[0][0][1], acc[0]);
+            acc[1] = fmaf(y, c[0][0][2] + c[0][0][3], acc[1]);
+        }
+        if (t == 0) { s_sum[warp][g] = acc[0]; s_sum[warp][8 + g] = acc[1]; }
+        __syncthreads();
+        const int col = r * 16 + threadIdx.x;
+        if (threadIdx.x < 16 && col < a.D) {
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < few::WARPS; ++w) v += s_sum[w][threadIdx.x];
+            const size_t at = size_t(tok) * a.ldy + col;
+            if (a.ytype == VELA_T_BF16) static_cast<__nv_bfloat16*>(a.Y)[at] = __float2bfloat16_rn(v);
+            else static_cast<__half*>(a.Y)[at] = __float2half_rn(v);
+        }
+        __syncthreads();
+    }
+}
+
 // Waits until all blocks of the grid have come here; false (and the error word set) if they have not within the limit.
 __device__ __forceinline__ bool grid_barrier(unsigned* count, unsigned want, unsigned* err, long long limit, int* flag) {
     __syncthreads();
     if (threadIdx.x == 0) {
         *flag = 1;
-        __threadfence();
-        atomicAdd(count, 1u);
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" :: "l"(count) : "memory");
         const long long t0 = clock64();
-        while (*reinterpret_cast<volatile unsigned*>(count) < want)
+        while (true) {
+            unsigned seen;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(count) : "memory");
+            if (seen >= want) break;
             if (clock64() - t0 > limit) { atomicCAS(err, 0u, unsigned(DEVERR_TIMEOUT_OTHER)); *flag = 0; break; }
-        __threadfence();
+        }
     }
     __syncthreads();
     return *flag != 0;
@@ -173,6 +335,7 @@ template <int NT, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS *
     int32_t* s_first = s_expert + P;
     int32_t* s_cnt = s_first + P + 1;
     int32_t* s_at = s_cnt + a.E;
+    int32_t* s_tok = s_at + P;                      // their tokens
     if (warp == 0) {
         for (int e = lane; e < a.E; e += 32) s_cnt[e] = 0;
         __syncwarp();
@@ -201,22 +364,24 @@ template <int NT, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS *
         }
         if (lane == 0) { s_n = n; s_first[n] = at; }
         __syncwarp();
-        for (int i0 = 0; i0 < P; i0 += 32) { const int i = i0 + lane; if (i < P) s_at[s_cnt[s_ids[i]] + s_list[i]] = i; }
+        for (int i0 = 0; i0 < P; i0 += 32) { const int i = i0 + lane; if (i < P) { const int q = s_cnt[s_ids[i]] + s_list[i]; s_at[q] = i; s_tok[q] = w4::quot(i, a.topk); } }
     }
     __syncthreads();
     const int V = s_n;
     // Runs of items: this block's row tiles of one slot after another.  ask: a run's weights on their way to the L2 cache, 64 KB of them at most
     auto ask = [&](const w4::Weights& W, int it, int hi) {
         if (threadIdx.x == 0 && it < hi) {
-            const int rt = w4::row_tiles(W), v = it / rt, n = min(min(hi - it, rt - (it - v * rt)), max(1, 65536 / (W.kt * 512)));
+            const int rt = w4::row_tiles(W), v = w4::quot(it, rt), n = min(min(hi - it, rt - (it - v * rt)), max(1, 65536 / (W.kt * 512)));
             w4::prefetch_l2(W.q + (size_t(s_expert[v]) * rt + (it - v * rt)) * W.kt * 32, min(n * W.kt * 512, 65536));
         }
     };
+    // the first of the V * rt items that are block b's
+    auto share = [&](int rt, int b) { const int q = w4::quot(V * rt, grid); return q * b + min(b, V * rt - q * grid); };
     auto runs = [&](const w4::Weights& W, auto run) {
         const int rt = w4::row_tiles(W);
-        const int lo = int((long long)V * rt * blockIdx.x / grid), hi = int((long long)V * rt * (blockIdx.x + 1) / grid);
+        const int lo = share(rt, blockIdx.x), hi = share(rt, blockIdx.x + 1);
         for (int it = lo; it < hi;) {
-            const int v = it / rt, r0 = it - v * rt, n = min(rt - r0, hi - it);
+            const int v = w4::quot(it, rt), r0 = it - v * rt, n = min(rt - r0, hi - it);
             it += n;
             ask(W, it, hi);
             run(v, size_t(s_expert[v]) * rt, r0, r0 + n, s_first[v + 1] - s_first[v]);
@@ -224,22 +389,23 @@ template <int NT, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS *
     };
     auto pair_of = [&](int v, int col) { return s_at[s_first[v] + col]; };
 
+    ask(a.up, share(w4::row_tiles(a.up), blockIdx.x), share(w4::row_tiles(a.up), blockIdx.x + 1));
     runs(a.up, [&](int v, size_t tile0, int r0, int r1, int c) {
-        const int nu = w4::units(a.up), room = a.room / c;
-        w4::stream<w4::F, NT, NT == 1 && FOLD == 128 ? 2 : 1, FOLD, ZERO, true>(a.up, tile0, r0, r1, c, sums, room,
+        const int nu = w4::units(a.up), room = w4::quot(a.room, c);
+        w4::stream<w4::F, NT, NT == 1 && FOLD == 128 ? 2 : 1, FOLD, ZERO, true>(a.up, tile0, r0, r1, c, a.split_up, sums, room,
             [&](int n, int u, uint32_t (&b)[16], w4::Pairs<FOLD>& p) {
-                auto at = [&](int col) { return size_t(a.t0 + pair_of(v, min(8 * n + col, c - 1)) / a.topk) * nu + u; };     // any row where there is none: its column is not used
+                auto at = [&](int col) { return size_t(a.t0 + s_tok[s_first[v] + min(8 * n + col, c - 1)]) * nu + u; };     // any row where there is none: its column is not used
                 w4::load_staged<FOLD>(b, p, a.xs + at(g) * 128 + 8 * t, a.xp + at(2 * t) * (128 / FOLD), a.xp + at(2 * t + 1) * (128 / FOLD));
             },
             [&](int rt, int col, int i, float gate, float up) { a.h[size_t(pair_of(v, col)) * a.I + rt * 8 + i] = gate / (1.f + expf(-gate)) * up; });
     });
     unsigned* count = a.count + a.t0 / T_BLOCK * COUNTERS;
-    ask(a.down, int((long long)V * w4::row_tiles(a.down) * blockIdx.x / grid), int((long long)V * w4::row_tiles(a.down) * (blockIdx.x + 1) / grid));
+    ask(a.down, share(w4::row_tiles(a.down), blockIdx.x), share(w4::row_tiles(a.down), blockIdx.x + 1));
     if (!grid_barrier(count, grid + a.extra, a.err, a.limit, &s_flag)) return;
 
     const int wide = w4::row_tiles(a.down) * 16;
     runs(a.down, [&](int v, size_t tile0, int r0, int r1, int c) {
-        w4::stream<w4::H, NT, 1, FOLD, ZERO, false>(a.down, tile0, r0, r1, c, sums, a.room / c,
+        w4::stream<w4::H, NT, 1, FOLD, ZERO, false>(a.down, tile0, r0, r1, c, a.split_down, sums, w4::quot(a.room, c),
             [&](int n, int u, uint32_t (&b)[32], w4::Pairs<FOLD>& p) {
                 w4::load_floats<FOLD>(b, p, a.h + size_t(pair_of(v, min(8 * n + g, c - 1))) * a.I + u * 128 + 8 * t, a.I - u * 128 - 8 * t, t);
             },
@@ -248,7 +414,7 @@ template <int NT, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS *
     if (!grid_barrier(count + 1, grid + a.extra, a.err, a.limit, &s_flag)) return;
 
     for (int i = blockIdx.x * (WARPS * 32) + threadIdx.x; i < a.tn * a.D; i += grid * (WARPS * 32)) {
-        const int tok = i / a.D, n = i - tok * a.D;
+        const int tok = w4::quot(i, a.D), n = i - tok * a.D;
         float y = 0.f;
         for (int j = 0; j < a.topk; ++j)
             y = fmaf(__ldg(a.weights + size_t(a.t0 + tok) * a.topk + j), __ldcg(a.o + size_t(tok * a.topk + j) * wide + n), y);
@@ -258,7 +424,7 @@ template <int NT, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS *
     }
 }
 
-struct Layout { size_t ids, weights, xs, xp, h, o, count, bytes; };
+struct Layout { size_t ids, weights, xs, xp, h, o, hi, lo, count, bytes; };
 Layout layout(const vela_moe& L, int T) {
     Layout w;
     const size_t n = size_t(T) * L.topk, nu = (size_t(L.D) + 127) / 128, fold = 128 / L.gate_up.group, some = size_t(std::min(T, T_BLOCK)) * L.topk;
@@ -267,6 +433,9 @@ Layout layout(const vela_moe& L, int T) {
     w.ids = take(n * 4); w.weights = take(n * 4);
     w.xs = take(T * nu * 256); w.xp = take(T * nu * fold * 8);
     w.h = take(some * L.I * 4); w.o = take(some * ((size_t(L.D) + 15) / 16 * 16) * 4);
+    // few tokens' rows: small, so always there
+    const size_t rows = size_t(few::PAIRS) * ((size_t(L.I) + 127) / 128) * 256;
+    w.hi = take(rows); w.lo = take(rows);
     w.count = take((size_t(T) + T_BLOCK - 1) / T_BLOCK * COUNTERS * 4);
     w.bytes = at;
     return w;
@@ -285,17 +454,47 @@ void check(const vela_moe& L, int T) {
 
 template <int NT, int FOLD, bool ZERO> void launch_experts(cudaStream_t st, MoeArgs a) {
     auto* kernel = expert_kernel<NT, FOLD, ZERO>;
+    // as many experts as the tokens reach on average
+    const int grid = sm_count();
+    const double slots = a.E * (1 - std::pow(1 - double(a.topk) / a.E, a.tn));
+    auto run = [&](const w4::Weights& W) { return std::min(w4::row_tiles(W), std::max(1, int(slots * w4::row_tiles(W) / grid))); };
+    a.split_up = w4::plan(w4::units(a.up), NT == 1 && FOLD == 128 ? 2 : 1, run(a.up));
+    a.split_down = w4::plan(w4::units(a.down), 1, run(a.down));
     // room for the sums of so many columns times rounds, then the slots
     a.room = NT == 1 ? 96 : 48;
     a.room_bytes = int(w4::sum_bytes(1, a.room));
-    const size_t smem = a.room_bytes + (size_t(a.tn) * a.topk * 5 + 1 + a.E) * 4;
-    constexpr size_t most = w4::sum_bytes(1, 96) + (size_t(T_BLOCK) * K_MAX * 5 + 1 + E_MAX) * 4;
+    const size_t smem = a.room_bytes + (size_t(a.tn) * a.topk * 6 + 1 + a.E) * 4;
+    constexpr size_t most = w4::sum_bytes(1, 96) + (size_t(T_BLOCK) * K_MAX * 6 + 1 + E_MAX) * 4;
     static std::atomic<int> ready[64];
     once_per_device(ready, [&] { VELA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most))); });
     void* args[] = {&a};
-    VELA_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kernel), dim3(sm_count()), dim3(WARPS * 32), args, smem, st));
+    VELA_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kernel), dim3(grid), dim3(WARPS * 32), args, smem, st));
+}
+template <class X, int FOLD, bool ZERO> void launch_few(cudaStream_t st, MoeArgs a) {
+    auto* up = few_up_kernel<X, FOLD, ZERO>;
+    const size_t smem = few::up_bytes<FOLD>(a.T, w4::units(a.up), a.E);
+    static std::atomic<int> ready[64];
+    once_per_device(ready, [&] { VELA_CUDA(cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM)); });
+    // whole clusters; all of a block's items in one round if there are warps for it, since a round costs a memory latency
+    const int blocks = 2 * sm_count(), items = a.T * a.topk * w4::row_tiles(a.up), grid = std::min(ceil_div(items, few::RANKS), std::max(1, blocks / few::RANKS)) * few::RANKS;
+    const int ks = std::max(1, std::min(w4::units(a.up), few::WARPS / ceil_div(items, grid)));
+    a.split_up = w4::Split{ks, few::WARPS / ks, 1};
+    up<<<grid, few::WARPS * 32, smem, st>>>(a);
+    few_down_kernel<FOLD, ZERO><<<std::min(a.T * w4::row_tiles(a.down), blocks), few::WARPS * 32, 0, st>>>(a);
+}
+template <int FOLD> void launch_few(cudaStream_t st, const MoeArgs& a) {
+    if (a.ytype == VELA_T_BF16) a.up.zero ? launch_few<__nv_bfloat16, FOLD, true>(st, a) : launch_few<__nv_bfloat16, FOLD, false>(st, a);
+    else a.up.zero ? launch_few<__half, FOLD, true>(st, a) : launch_few<__half, FOLD, false>(st, a);
+}
+// Which form.  Measured over 1 to 8 tokens, widths 512 to 4096, 8 to 128 experts of 256 to 2048 (units: gate and up units of 128 columns for each SM): the few-token form takes
+// 7.5 to 23 us against 16 to 26 of the other up to 64 units, loses above (T = 8, 129 units: 31 against 26), and with one token, where no weight is shared, still wins at 166 (27 against 30).
+template <int FOLD> bool is_few(const MoeArgs& a, int router_type) {
+    const double units = double(a.T) * a.topk * w4::row_tiles(a.up) * w4::units(a.up) / sm_count();
+    return units <= (a.T == 1 ? 192 : 64) && a.T <= few::TOKENS && a.E <= few::EXPERTS && a.T * a.topk <= few::PAIRS && router_type == a.ytype && a.vecx && a.vecr &&
+           size_t(a.E) * a.D <= FEW_ROUTER && few::up_bytes<FOLD>(a.T, w4::units(a.up), a.E) <= FEW_SMEM && !a.extra;
 }
 template <int FOLD> void launch(cudaStream_t st, MoeArgs a, int router_type) {
+    if (is_few<FOLD>(a, router_type)) return launch_few<FOLD>(st, a);
     const dim3 grid(RANKS, a.T);
     if (a.ytype == VELA_T_BF16) {
         if (router_type == VELA_T_F32) route_kernel<__nv_bfloat16, float, FOLD><<<grid, ROUTE_WARPS * 32, 0, st>>>(a);
@@ -336,6 +535,8 @@ void moe_w4(cudaStream_t st, int type, const void* X, int ldx, int T, const vela
     a.xp = reinterpret_cast<float2*>(w + o.xp);
     a.h = reinterpret_cast<float*>(w + o.h);
     a.o = reinterpret_cast<float*>(w + o.o);
+    a.hi = reinterpret_cast<__nv_bfloat16*>(w + o.hi);
+    a.lo = reinterpret_cast<__nv_bfloat16*>(w + o.lo);
     a.count = reinterpret_cast<unsigned*>(w + o.count);
     a.D = L.D; a.I = L.I; a.E = L.E; a.topk = L.topk; a.T = T; a.ldx = ldx; a.ldy = ldy; a.score = L.score; a.renorm = L.renorm; a.scale = L.scale;
     a.ytype = type;

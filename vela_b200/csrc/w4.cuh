@@ -77,6 +77,14 @@ template <class M> __device__ __forceinline__ Consts consts() {
 }
 template <> __device__ __forceinline__ Consts consts<int8_t>() { return Consts{}; }
 
+// a / b for a >= 0, b > 0: the quotient of floats is off by a few at most, which the loops put right (a division of integers takes many times as long)
+__device__ __forceinline__ int quot(int a, int b) {
+    int q = int(__fdividef(float(a), float(b))), r = a - q * b;
+    while (r < 0) { --q; r += b; }
+    while (r >= b) { ++q; r -= b; }
+    return q;
+}
+
 // the pair (row g, row g + 8) of scales as floats
 __device__ __forceinline__ float2 scale_pair(uint32_t u, bool f16) {
     if (f16) return __half22float2(*reinterpret_cast<__half2*>(&u));

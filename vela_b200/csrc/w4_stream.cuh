@@ -145,26 +145,32 @@ constexpr int COL = 20;                   // floats from one column's 16 sums to
 constexpr size_t SUMS = 160 * 1024;       // bytes of shared memory for sums, at most
 __host__ __device__ constexpr size_t sum_bytes(int cols, int rounds) { return size_t(WARPS) * cols * COL * 4 * rounds; }
 
+// How a block splits a product: ks warps share out the units of a row tile, UW to each at a time (a chunk; several where there are more), and the block takes slots = WARPS / ks
+// row tiles in a round.  The split with the least time for runs of about nrow row tiles: a chunk costs its rounds and about two more to bring the activations.
+struct Split { int ks, slots, chunks; };
+inline Split plan(int nu, int uw, int nrow) {
+    Split best{1, WARPS, nu};
+    long long cost = 0;
+    for (int ks = 1; ks <= WARPS && (ks == 1 || (ks - 1) * uw < nu); ++ks) {
+        const Split s{ks, WARPS / ks, (nu + ks * uw - 1) / (ks * uw)};
+        const long long c = (long long)((nrow + s.slots - 1) / s.slots + 2) * s.chunks;
+        if (ks == 1 || c < cost) { best = s; cost = c; }
+    }
+    return best;
+}
+
 // The block's share: row tiles r0 .. r1 - 1 (at least one) of a matrix whose first row tile is number tile0, against `cols` <= 8 NT activation rows.
-// ks warps share out the units of a row tile, UW to each at a time (a chunk; several where there are more), and the block takes
-// WARPS / ks row tiles in a round.  Weights are loaded one round ahead.  A warp's sums go to shared memory and are added there, in the order of the warps, once for `room`
+// Weights are loaded one round ahead.  A warp's sums go to shared memory and are added there, in the order of the warps, once for `room`
 // rounds (sum_bytes).  load(n, u, b, pairs): operands of column tile n, unit u, by a whole warp; out(rt, col, row or half row, sums):
 // called by one thread for each row of 16, or with PAIRED for each i < 8 with the sums of rows i and i + 8.
 template <Kind KIND, int NT, int UW, int FOLD, bool ZERO, bool PAIRED, class LOAD, class OUT>
-__device__ __forceinline__ void stream(const Weights& W, size_t tile0, int r0, int r1, int cols, float* sums, int room, LOAD load, OUT out) {
+__device__ __forceinline__ void stream(const Weights& W, size_t tile0, int r0, int r1, int cols, const Split& split, float* sums, int room, LOAD load, OUT out) {
     typedef Unit<FOLD, ZERO> U;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int nu = units(W), nrow = r1 - r0, per = 7 - W.gshift;
-    // The split with the least time: each lane tries one ks.  A chunk costs its rounds and about two more to bring the activations.
-    int ks;
-    {
-        const int k = (lane & 15) + 1, c = (nu + k * UW - 1) / (k * UW), r = (nrow + WARPS / k - 1) / (WARPS / k);
-        const unsigned cost = k == 1 || (k - 1) * UW < nu ? unsigned(min((r + 2) * c, 1 << 26)) : 1u << 26;
-        ks = int(__reduce_min_sync(0xffffffffu, cost << 5 | unsigned(k)) & 31u);
-    }
-    const int chunks = (nu + ks * UW - 1) / (ks * UW), slots = WARPS / ks, sl = warp / ks, kw = warp - sl * ks;
-    const int total = (nrow - sl + slots - 1) / slots;      // of this warp, if it has a slot
-    const int rounds = (nrow + slots - 1) / slots, most = min(rounds, room);
+    const int ks = split.ks, slots = split.slots, chunks = split.chunks, sl = quot(warp, ks), kw = warp - sl * ks;
+    const int total = quot(max(nrow - sl + slots - 1, 0), slots);      // of this warp, if it has a slot
+    const int rounds = quot(nrow + slots - 1, slots), most = min(rounds, room);
     float* const mine = sums + size_t(warp) * most * cols * COL;
     auto count = [&](int base, int n) { return sl < slots ? max(0, min(n, total - base)) : 0; };      // rounds with a row tile for this warp
 
@@ -269,14 +275,15 @@ __device__ __forceinline__ void stream(const Weights& W, size_t tile0, int r0, i
         }
         __syncthreads();
         constexpr int ROWS = PAIRED ? 8 : 16;
-        const int each = cols * ROWS;                       // values of a row tile
-        for (int i = threadIdx.x; i < n * slots * each; i += WARPS * 32) {
-            const int rr = i / each, q = i - rr * each, col = q / ROWS, row = q % ROWS, jj = rr / slots, s = rr - jj * slots;
-            const int rt = r0 + (base + jj) * slots + s;
+        // thread i sums row i mod ROWS of every WARPS * 32 / ROWS-th column of a row tile
+        const int row = threadIdx.x % ROWS;
+        for (int i = threadIdx.x / ROWS; i < n * slots * cols; i += WARPS * 32 / ROWS) {
+            const int rr = quot(i, cols), col = i - rr * cols, jj = quot(rr, slots), s = rr - jj * slots, rt = r0 + (base + jj) * slots + s;
             if (rt >= r1) continue;
-            const float* e = sums + (size_t(s * ks) * most + jj) * cols * COL + col * COL + row;
+            const float* e = sums + ((s * ks * most + jj) * cols + col) * COL + row;
             float v = 0.f, w = 0.f;
-            for (int k = 0; k < ks; ++k) { v += e[0]; if (PAIRED) w += e[8]; e += size_t(most) * cols * COL; }
+#pragma unroll 4
+            for (int k = 0; k < ks; ++k) { v += e[0]; if (PAIRED) w += e[8]; e += most * cols * COL; }
             out(rt, col, row, v, w);
         }
         __syncthreads();
