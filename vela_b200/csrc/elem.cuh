@@ -26,34 +26,71 @@ template <> struct Elem<float> {
     static __device__ __forceinline__ float put(float v) { return v; }
 };
 
-// v[i] = p[i] for i < n <= 8, 0 beyond; `vec`: n == 8 and p aligned to its 8 elements (at most 16 bytes)
-template <class T> __device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
+// 8 neighbouring values as they lie in memory
+template <class T> union Raw8 {
+    uint4 u[sizeof(T) / 2];
+    T e[8];
+    __device__ __forceinline__ Raw8() {}
+};
+// p[i] for i < n <= 8, zero bits beyond; `vec`: n == 8 and p aligned to 16 bytes
+template <class T> __device__ __forceinline__ void load_raw(Raw8<T>& x, const T* p, int n, bool vec) {
     if (vec) {
-        constexpr int W = sizeof(T) * 8 / 16;        // 16-byte words
-        union { uint4 u[W]; T e[8]; } x;
 #pragma unroll
-        for (int i = 0; i < W; ++i) x.u[i] = reinterpret_cast<const uint4*>(p)[i];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = Elem<T>::get(x.e[i]);
+        for (int i = 0; i < int(sizeof(T) / 2); ++i) x.u[i] = reinterpret_cast<const uint4*>(p)[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? Elem<T>::get(p[i]) : 0.f;
+        for (int i = 0; i < int(sizeof(T) / 2); ++i) x.u[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) if (i < n) x.e[i] = p[i];
     }
 }
-template <class T> __device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
-    if (vec) {
-        constexpr int W = sizeof(T) * 8 / 16;
-        union { uint4 u[W]; T e[8]; } x;
+// x as floats
+template <class T> __device__ __forceinline__ void unpack8(float (&v)[8], const Raw8<T>& x) {
+    if constexpr (Elem<T>::code == VELA_T_BF16) {
+        const uint32_t w[4] = {x.u[0].x, x.u[0].y, x.u[0].z, x.u[0].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x.e[i] = Elem<T>::put(v[i]);
+        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    } else if constexpr (Elem<T>::code == VELA_T_F16) {
+        const uint32_t w[4] = {x.u[0].x, x.u[0].y, x.u[0].z, x.u[0].w};
 #pragma unroll
-        for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(p)[i] = x.u[i];
+        for (int i = 0; i < 4; ++i) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i])); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) if (i < n) p[i] = Elem<T>::put(v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = Elem<T>::get(x.e[i]);
     }
 }
 
+// the same as floats
+template <class T> __device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
+    Raw8<T> x;
+    load_raw(x, p, n, vec);
+    unpack8(v, x);
+}
+// v as T, two at a time where T is narrower than a float (one instruction then)
+template <class T> __device__ __forceinline__ void pack8(Raw8<T>& x, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (Elem<T>::code == VELA_T_BF16) { const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&p); }
+            else { const __half2 p = __floats2half2_rn(v[2 * i], v[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&p); }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x.e[i] = Elem<T>::put(v[i]);
+    }
+}
+template <class T> __device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
+    Raw8<T> x;
+    pack8(x, v);
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < int(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = x.u[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) if (i < n) p[i] = x.e[i];
+    }
+}
 // the larger of two, a NaN where either is one
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;

@@ -13,30 +13,23 @@ constexpr float AMAX_MIN = 1e-30f;     // the scale of an all-zero row or group:
 
 struct NormArgs {
     const void* X; const void* R; const void* g; void* S; void* Y; void* Q; float* qscale;
-    int ldx, ldr, lds, ldy, ldq, M, C, qgroup, ngroups;
+    int ldx, ldr, lds, ldy, ldq, M, C, qgroup, ngroups, gshift, gmask;      // log2 of the group and the group - 1; one group: 31, all bits
     float eps;
 };
 
-template <int THREADS> __device__ __forceinline__ float block_sum(float v, float* red) {
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (THREADS == 32) return v;
-    __syncthreads();
+// over a warp, or over the block through `red` (a word for each warp, not used by the block for anything else)
+template <bool WARP, class OP> __device__ __forceinline__ float reduce(float v, float* red, OP op) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (WARP) return v;
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    float s = 0.f;
-    for (int i = 0; i < THREADS / 32; ++i) s += red[i];
-    return s;
+    v = red[0];
+    for (int i = 1; i < int(blockDim.x >> 5); ++i) v = op(v, red[i]);
+    return v;
 }
-template <int THREADS> __device__ __forceinline__ float block_max(float v, float* red) {
-    for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (THREADS == 32) return v;
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float s = 0.f;
-    for (int i = 0; i < THREADS / 32; ++i) s = max_nan(s, red[i]);
-    return s;
-}
+struct Sum { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+struct Max { __device__ __forceinline__ float operator()(float a, float b) const { return max_nan(a, b); } };
 
 // 8 values of q = y * inv as bytes
 template <int QT> __device__ __forceinline__ void store_q8(uint8_t* p, int n, bool vec, const float (&y)[8], float inv) {
@@ -54,71 +47,77 @@ template <int QT> __device__ __forceinline__ void store_q8(uint8_t* p, int n, bo
         for (int i = 0; i < 8; ++i) if (i < n) p[i] = o.b[i];
 }
 
-// One block of THREADS threads for each row; thread i holds values 8 (i + j THREADS) .. + 7, j < V, in registers.
-// The group of 64 or 128 columns is 8 or 16 neighbouring lanes.
-template <class T, int QT, int THREADS, int V> __global__ void __launch_bounds__(THREADS) rms_norm_kernel(NormArgs a, bool vec) {
-    __shared__ float red[THREADS / 32 + 1];
+// A block, or with WARP a warp, for each row; thread i holds values 8 (i + j n) .. + 7, j < V, in registers, n the row's threads.  All three inputs are fetched
+// before the first reduction.  The group of 64 or 128 columns is 8 or 16 neighbouring lanes.  VEC: rows are whole and aligned vectors.
+template <class T, int QT, int V, bool WARP, bool VEC> __global__ void __launch_bounds__(WARP ? 256 : 512) rms_norm_kernel(const NormArgs a) {
+    __shared__ float red[2][16];
     constexpr float TOP = QT == VELA_T_I8 ? 127.f : 448.f;
-    const size_t row = blockIdx.x;
+    const int n = WARP ? 32 : blockDim.x, ti = WARP ? threadIdx.x & 31 : threadIdx.x;
+    const size_t row = WARP ? size_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+    if (WARP && row >= size_t(a.M)) return;
     const T* x = static_cast<const T*>(a.X) + row * a.ldx;
-    const T* r = a.R ? static_cast<const T*>(a.R) + row * a.ldr : nullptr;
+    const T* r = static_cast<const T*>(a.R) + row * a.ldr;
     const T* g = static_cast<const T*>(a.g);
+    Raw8<T> rx[V], rr[V], rg[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = 8 * (ti + j * n), left = a.C - c;
+        if (left <= 0) { load_raw(rx[j], x, 0, false); load_raw(rr[j], x, 0, false); load_raw(rg[j], g, 0, false); continue; }
+        load_raw(rx[j], x + c, left, VEC);
+        if (a.R) load_raw(rr[j], r + c, left, VEC);
+        load_raw(rg[j], g + c, left, VEC);
+    }
     float h[V][8];
     float ss = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = 8 * (int(threadIdx.x) + j * THREADS), n = min(8, a.C - c);
-        if (n <= 0) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) h[j][i] = 0.f;
-            continue;
-        }
-        load8(x + c, n, vec, h[j]);
-        if (r) {
+        const int c = 8 * (ti + j * n);
+        unpack8(h[j], rx[j]);
+        if (a.R) {
             float t[8];
-            load8(r + c, n, vec, t);
+            unpack8(t, rr[j]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[j][i] += t[i];
         }
-        if (a.S) store8(static_cast<T*>(a.S) + row * a.lds + c, n, vec, h[j]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(h[j][i], h[j][i], ss);
+        if (a.S && c < a.C) store8(static_cast<T*>(a.S) + row * a.lds + c, a.C - c, VEC, h[j]);
     }
-    const float rstd = rsqrtf(block_sum<THREADS>(ss, red) / float(a.C) + a.eps);
-    float top = 0.f;
-    float am[V];
+    const float rstd = rsqrtf(reduce<WARP>(ss, red[0], Sum()) / float(a.C) + a.eps);
+    float top = 0.f, am[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = 8 * (int(threadIdx.x) + j * THREADS), n = min(8, a.C - c);
-        am[j] = 0.f;
-        if (n <= 0) continue;
+        const int c = 8 * (ti + j * n);
         float t[8];
-        load8(g + c, n, vec, t);
+        unpack8(t, rg[j]);
+        am[j] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { h[j][i] = h[j][i] * rstd * t[i]; if (i < n) am[j] = max_nan(am[j], fabsf(h[j][i])); }
-        if (a.Y) store8(static_cast<T*>(a.Y) + row * a.ldy + c, n, vec, h[j]);
+        for (int i = 0; i < 8; ++i) { h[j][i] = h[j][i] * rstd * t[i]; if (VEC || c + i < a.C) am[j] = max_nan(am[j], fabsf(h[j][i])); }
+        if (VEC && c >= a.C) am[j] = 0.f;
+        if (a.Y && c < a.C) store8(static_cast<T*>(a.Y) + row * a.ldy + c, a.C - c, VEC, h[j]);
         top = max_nan(top, am[j]);
     }
     if (!a.Q) return;
-    if (a.qgroup == 0) top = block_max<THREADS>(top, red);
+    if (a.qgroup == 0) top = reduce<WARP>(top, red[1], Max());
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = 8 * (int(threadIdx.x) + j * THREADS), n = min(8, a.C - c);
+        const int c = 8 * (ti + j * n);
         float m = top;
         if (a.qgroup) {
             m = am[j];
-            for (int o = 1; o < a.qgroup / 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (a.gshift == 7) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 8));
         }
-        if (n <= 0) continue;
+        if (c >= a.C) continue;
         m = m < AMAX_MIN ? AMAX_MIN : m;
-        if (a.qgroup ? c % a.qgroup == 0 : c == 0) a.qscale[row * a.ngroups + (a.qgroup ? c / a.qgroup : 0)] = m / TOP;
-        store_q8<QT>(static_cast<uint8_t*>(a.Q) + row * a.ldq + c, n, vec, h[j], TOP / m);
+        if ((c & a.gmask) == 0) a.qscale[row * a.ngroups + (c >> a.gshift)] = m * (1.f / TOP);
+        store_q8<QT>(static_cast<uint8_t*>(a.Q) + row * a.ldq + c, a.C - c, VEC, h[j], TOP / m);
     }
 }
 
 // Rows too long for the registers: the inputs are read again for each step.  S is written last, since it may be X or R.
-template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREADS) rms_norm_long_kernel(NormArgs a, bool vec) {
-    __shared__ float red[THREADS / 32 + 1];
+template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREADS) rms_norm_long_kernel(const NormArgs a, bool vec) {
+    __shared__ float red[2][THREADS / 32];
     constexpr float TOP = QT == VELA_T_I8 ? 127.f : 448.f;
     const size_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.X) + row * a.ldx;
@@ -140,7 +139,7 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(h[i], h[i], ss);
     }
-    const float rstd = rsqrtf(block_sum<THREADS>(ss, red) / float(a.C) + a.eps);
+    const float rstd = rsqrtf(reduce<false>(ss, red[0], Sum()) / float(a.C) + a.eps);
     float top = 0.f;
     if (a.Q && a.qgroup == 0) {
         for (int c = 8 * threadIdx.x; c < a.C; c += 8 * THREADS) {
@@ -151,7 +150,7 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
 #pragma unroll
             for (int i = 0; i < 8; ++i) if (i < n) top = max_nan(top, fabsf(h[i] * rstd * t[i]));
         }
-        top = block_max<THREADS>(top, red);
+        top = reduce<false>(top, red[1], Max());
     }
     for (int c0 = 0; c0 < a.C; c0 += 8 * THREADS) {
         const int c = c0 + 8 * int(threadIdx.x), n = min(8, a.C - c);
@@ -170,20 +169,25 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
         else m = top;
         if (n <= 0) continue;
         m = m < AMAX_MIN ? AMAX_MIN : m;
-        if (a.qgroup ? c % a.qgroup == 0 : c == 0) a.qscale[row * a.ngroups + (a.qgroup ? c / a.qgroup : 0)] = m / TOP;
+        if ((c & a.gmask) == 0) a.qscale[row * a.ngroups + (c >> a.gshift)] = m * (1.f / TOP);
         store_q8<QT>(static_cast<uint8_t*>(a.Q) + row * a.ldq + c, n, vec, h, TOP / m);
     }
 }
 
-template <class T, int QT> void launch(cudaStream_t st, const NormArgs& a, bool vec) {
-    const int nv = ceil_div(a.C, 8);
-    if (nv <= 128) rms_norm_kernel<T, QT, 128, 1><<<a.M, 128, 0, st>>>(a, vec);
-    else if (nv <= 256) rms_norm_kernel<T, QT, 256, 1><<<a.M, 256, 0, st>>>(a, vec);
-    else if (nv <= 512) rms_norm_kernel<T, QT, 256, 2><<<a.M, 256, 0, st>>>(a, vec);
-    else if (nv <= 1024) rms_norm_kernel<T, QT, 512, 2><<<a.M, 512, 0, st>>>(a, vec);
-    else if (nv <= 2048) rms_norm_kernel<T, QT, 512, 4><<<a.M, 512, 0, st>>>(a, vec);
-    else rms_norm_long_kernel<T, QT, 512><<<a.M, 512, 0, st>>>(a, vec);
+// A warp a row for short rows (without a block's meeting; up to 1024 columns only where there are rows enough to hide that each warp then takes 4 vectors one after another:
+// 77 rows of 1024 take 4.8 us so and 2.4 by blocks), else a block of as many threads as the row has pairs of vectors, so that few of them idle.
+template <class T, int QT, bool VEC> void launch(cudaStream_t st, const NormArgs& a) {
+    const int nv = ceil_div(a.C, 8), warps = 8;
+    auto block = [&](int v) { return ceil_div(ceil_div(nv, v), 32) * 32; };
+    if (nv <= 32) rms_norm_kernel<T, QT, 1, true, VEC><<<ceil_div(a.M, warps), 32 * warps, 0, st>>>(a);
+    else if (nv <= 64) rms_norm_kernel<T, QT, 2, true, VEC><<<ceil_div(a.M, warps), 32 * warps, 0, st>>>(a);
+    else if (nv <= 128 && a.M >= 4096) rms_norm_kernel<T, QT, 4, true, VEC><<<ceil_div(a.M, warps), 32 * warps, 0, st>>>(a);
+    else if (nv <= 512 && a.M <= 128) rms_norm_kernel<T, QT, 1, false, VEC><<<a.M, block(1), 0, st>>>(a);
+    else if (nv <= 1024) rms_norm_kernel<T, QT, 2, false, VEC><<<a.M, block(2), 0, st>>>(a);
+    else if (nv <= 2048) rms_norm_kernel<T, QT, 4, false, VEC><<<a.M, block(4), 0, st>>>(a);
+    else rms_norm_long_kernel<T, QT, 512><<<a.M, 512, 0, st>>>(a, VEC);
 }
+template <class T, int QT> void launch(cudaStream_t st, const NormArgs& a, bool vec) { vec ? launch<T, QT, true>(st, a) : launch<T, QT, false>(st, a); }
 
 void rms_norm_q8(cudaStream_t st, int type, const NormArgs& a, int qtype) {
     VELA_REQUIRE(type == VELA_T_BF16 || type == VELA_T_F16 || type == VELA_T_F32, "rms_norm_q8: type must be bf16, f16 or f32");
@@ -217,7 +221,7 @@ void rms_norm_q8(cudaStream_t st, int type, const NormArgs& a, int qtype) {
 extern "C" int vela_rms_norm_q8(void* stream, int type, const void* X, int ldx, const void* R, int ldr, const void* g, float eps, int M, int C,
                                 void* S, int lds, void* Y, int ldy, int qtype, void* Q, int ldq, float* qscale, int qgroup) {
     return vela::guarded("vela_rms_norm_q8", [&] {
-        vela::NormArgs a{X, R, g, S, Y, Q, qscale, ldx, ldr, lds, ldy, ldq, M, C, qgroup, qgroup > 0 ? (C - 1) / qgroup + 1 : 1, eps};
+        vela::NormArgs a{X, R, g, S, Y, Q, qscale, ldx, ldr, lds, ldy, ldq, M, C, qgroup, qgroup > 0 ? (C - 1) / qgroup + 1 : 1, qgroup == 64 ? 6 : qgroup == 128 ? 7 : 31, qgroup > 0 ? qgroup - 1 : -1, eps};
         vela::rms_norm_q8(static_cast<cudaStream_t>(stream), type, a, qtype);
     });
 }
