@@ -228,7 +228,7 @@ int vela_gemv_w4(void* stream, int xtype, const void* X, int ldx, const float* x
 /* A mixture-of-experts layer: p = softmax (score 0) or sigmoid (score 1) of X router^T; the topk largest p (+ select_bias,
  * used for the choice alone) are chosen, ties to the lower expert; their p, divided by their sum where renorm is set, times
  * `scale`, weigh the experts' outputs down_e (silu(gate_e x) * (up_e x)).
- * router [E][D] (the activations' type or f32); select_bias float [E] or NULL; E <= 1024, topk <= min(E, 32).
+ * router [E][D] (the activations' type or f32); select_bias float [E] or NULL; E <= 1024, topk <= min(E, 32); D, I <= 2^20.
  * gate_up: E matrices [2 I, D], one after another, I a multiple of 8: rows 16 i .. 16 i + 7 are gate rows 8 i .. 8 i + 7 and
  * rows 16 i + 8 .. 16 i + 15 the up rows of the same numbers.  down: E matrices [D, I].  Both vela_w4's N, K are one
  * expert's.  The hidden values are carried as the sum of two bf16 numbers (16 bits of precision). */
@@ -240,7 +240,7 @@ typedef struct vela_moe {
 } vela_moe;
 /* bytes of workspace for T tokens (0: arguments that vela_moe_w4 refuses).  Its contents need no preparation. */
 size_t vela_moe_w4_workspace(const vela_moe* L, int T);
-/* Y [T, D] = the layer's output for X [T, D] (`type` bf16 or f16).  ids [T][topk] int32 and weights [T][topk] float
+/* Y [T, D] = the layer's output for X [T, D] (`type` bf16 or f16), T <= 65535 (32 tokens at a time: the weights are read again for the next).  ids [T][topk] int32 and weights [T][topk] float
  * (largest first) are written where they are not NULL.  A NaN among a token's scores counts as the smallest score.
  * workspace: 16-byte aligned; calls that may overlap need one each. */
 int vela_moe_w4(void* stream, int type, const void* X, int ldx, int T, const vela_moe* L, void* Y, int ldy,

@@ -185,6 +185,41 @@ def test_streams_graphs_and_repeats():
     assert V.lib().vela_device_error(1) == 0
 
 
+@pytest.mark.parametrize("T,f32", [(1, False), (3, True), (20, False)])
+def test_two_streams_at_a_time(T, f32):
+    """both forms of the layer (few tokens with a router of their own type; else), on two streams with a workspace each"""
+    layer = Layer(14, 256, 64, 12, 3, abi.T_BF16, 64, router_f32=f32)
+    x = torch.randn(T, 256, device="cuda").bfloat16()
+    y = torch.empty_like(x)
+    wa = layer(x, y)
+    layer.check(x, y, None, None)
+    wb = torch.empty_like(wa)
+    ya, yb = torch.empty_like(x), torch.empty_like(x)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        layer(x, ya, stream=a.cuda_stream, ws=wa)
+        layer(x, yb, stream=b.cuda_stream, ws=wb)
+    torch.cuda.synchronize()
+    assert torch.equal(ya, y) and torch.equal(yb, y)
+    assert V.lib().vela_device_error(1) == 0
+
+
+def test_both_forms_agree():
+    """a router in 32 bits takes the form with a barrier, the same numbers in bf16 the form for few tokens"""
+    for T in (1, 4):
+        layer = Layer(16, 384, 136, 9, 2, abi.T_BF16, 128)
+        x = torch.randn(T, 384, device="cuda").bfloat16()
+        out = []
+        for f32 in (False, True):
+            layer.router = layer.router.float() if f32 else layer.router
+            y = torch.empty_like(x); ids = torch.empty(T, 2, dtype=torch.int32, device="cuda"); w = torch.empty(T, 2, device="cuda")
+            layer(x, y, ids, w)
+            layer.check(x, y, ids, w)
+            out.append(ids)
+        assert torch.equal(*out)
+
+
 def test_no_tokens():
     layer = Layer(11, 64, 16, 2, 1, abi.T_BF16, 64)
     x = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")

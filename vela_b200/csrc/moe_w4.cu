@@ -158,6 +158,7 @@ template <class X, int FOLD, bool ZERO> __global__ void __cluster_dims__(few::RA
     __shared__ __align__(16) uint32_t s_key[few::TOKENS][few::EXPERTS];
     __shared__ int32_t s_ids[few::PAIRS];
     __shared__ float s_sum[few::WARPS][16];
+    asm volatile("griddepcontrol.launch_dependents;");     // few_down_kernel may be brought up
     cg::cluster_group cluster = cg::this_cluster();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, nu = w4::units(a.up), rank = blockIdx.x % few::RANKS;
     const X* x = static_cast<const X*>(a.X);
@@ -273,6 +274,7 @@ template <int FOLD, bool ZERO> __global__ void __launch_bounds__(few::WARPS * 32
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rt = w4::row_tiles(a.down), nu = w4::units(a.down), items = a.T * rt, n = a.topk * nu, wide = nu * 128;
     const w4::Consts k = w4::consts<__nv_bfloat16>();
+    asm volatile("griddepcontrol.wait;" ::: "memory");     // few_up_kernel has ended and its results are visible
     // the two terms of a hidden value are columns 0 and 1 of the product (and 2 to 7 again, which are not used)
     const __nv_bfloat16* h = (g & 1 ? a.lo : a.hi) + 8 * t;
     for (int it = blockIdx.x; it < items; it += gridDim.x) {
@@ -443,7 +445,7 @@ Layout layout(const vela_moe& L, int T) {
 
 void check(const vela_moe& L, int T) {
     VELA_REQUIRE(T >= 0 && T <= 65535, "moe_w4: T must lie in 0 .. 65535");
-    VELA_REQUIRE(L.D > 0 && L.I > 0 && L.I % 8 == 0 && L.I <= (1 << 24) && L.D <= (1 << 24), "moe_w4: D > 0 and I a positive multiple of 8");
+    VELA_REQUIRE(L.D > 0 && L.I > 0 && L.I % 8 == 0 && L.I <= (1 << 20) && L.D <= (1 << 20), "moe_w4: D > 0 and I a positive multiple of 8, 2^20 at most");
     VELA_REQUIRE(L.E > 0 && L.E <= E_MAX && L.topk > 0 && L.topk <= K_MAX && L.topk <= L.E, "moe_w4: E in 1 .. 1024 and topk in 1 .. min(E, 32)");
     VELA_REQUIRE(L.score == 0 || L.score == 1, "moe_w4: score must be 0 (softmax) or 1 (sigmoid)");
     VELA_REQUIRE(L.gate_up.N == 2 * L.I && L.gate_up.K == L.D, "moe_w4: gate_up must be [2 I, D]");
@@ -480,7 +482,13 @@ template <class X, int FOLD, bool ZERO> void launch_few(cudaStream_t st, MoeArgs
     const int ks = std::max(1, std::min(w4::units(a.up), few::WARPS / ceil_div(items, grid)));
     a.split_up = w4::Split{ks, few::WARPS / ks, 1};
     up<<<grid, few::WARPS * 32, smem, st>>>(a);
-    few_down_kernel<FOLD, ZERO><<<std::min(a.T * w4::row_tiles(a.down), blocks), few::WARPS * 32, 0, st>>>(a);
+    // brought up while the first is still running; it waits for it before it reads anything
+    cudaLaunchAttribute at[1] = {};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(std::min(a.T * w4::row_tiles(a.down), blocks)); cfg.blockDim = dim3(few::WARPS * 32); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
+    VELA_CUDA(cudaLaunchKernelEx(&cfg, few_down_kernel<FOLD, ZERO>, a));
 }
 template <int FOLD> void launch_few(cudaStream_t st, const MoeArgs& a) {
     if (a.ytype == VELA_T_BF16) a.up.zero ? launch_few<__nv_bfloat16, FOLD, true>(st, a) : launch_few<__nv_bfloat16, FOLD, false>(st, a);
@@ -495,6 +503,7 @@ template <int FOLD> bool is_few(const MoeArgs& a, int router_type) {
 }
 template <int FOLD> void launch(cudaStream_t st, MoeArgs a, int router_type) {
     if (is_few<FOLD>(a, router_type)) return launch_few<FOLD>(st, a);
+    a.err = device_error_word(&g_moe_err);
     const dim3 grid(RANKS, a.T);
     if (a.ytype == VELA_T_BF16) {
         if (router_type == VELA_T_F32) route_kernel<__nv_bfloat16, float, FOLD><<<grid, ROUTE_WARPS * 32, 0, st>>>(a);
@@ -542,7 +551,6 @@ void moe_w4(cudaStream_t st, int type, const void* X, int ldx, int T, const vela
     a.ytype = type;
     a.vecx = L.D % 8 == 0 && ldx % 8 == 0 && aligned(X, 16);
     a.vecr = L.D % 8 == 0 && aligned(L.router, 16);
-    a.err = device_error_word(&g_moe_err);
     a.limit = limit > 0 ? limit : WAIT_LIMIT_CYCLES;
     a.extra = extra;
     if (L.gate_up.group == 32) launch<32>(st, a, L.router_type);
