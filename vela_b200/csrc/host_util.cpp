@@ -84,6 +84,29 @@ int blocks_per_sm(const void* kernel, int threads, size_t smem) {
     return n;
 }
 
+int clusters_per_device(const void* kernel, int cluster, int threads, size_t smem) {
+    struct Entry { int dev; const void* k; size_t smem; int clusters; };
+    static std::mutex mu;
+    static std::vector<Entry> cache;
+    smem = align_up(smem, 8192);                   // few entries, whatever the sizes
+    const int d = current_device();
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        for (const Entry& e : cache) if (e.dev == d && e.k == kernel && e.smem == smem) return e.clusters;
+    }
+    cudaLaunchAttribute at[1] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = unsigned(cluster); at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(cluster)); cfg.blockDim = dim3(unsigned(threads)); cfg.dynamicSmemBytes = smem; cfg.attrs = at; cfg.numAttrs = 1;
+    int n = 0;
+    VELA_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+    n = n > 0 ? n : 1;
+    std::lock_guard<std::mutex> lk(mu);
+    cache.push_back(Entry{d, kernel, smem, n});
+    return n;
+}
+
 void register_error_word(const void* symbol) {
     std::lock_guard<std::mutex> lk(g_mu);
     for (auto* s : g_symbols) if (s == symbol) return;

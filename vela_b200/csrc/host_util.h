@@ -33,6 +33,9 @@ int sm_count();
 // Blocks of `kernel` resident on one SM at `threads` threads and `smem` dynamic shared bytes (at least 1), on the
 // current device; cached.  Grids of this many blocks per SM run in one wave.
 int blocks_per_sm(const void* kernel, int threads, size_t smem);
+// Clusters of `kernel` (of `cluster` blocks each, `threads` threads, `smem` dynamic shared bytes) that the current device holds at a time
+// (at least 1); cached.  Fewer than blocks_per_sm would let one think: a cluster lies within a GPC, whose SMs need not be a multiple of it.
+int clusters_per_device(const void* kernel, int cluster, int threads, size_t smem);
 
 // Per-launch options of the kernels with bounded waits (GEMM, attention).
 struct LaunchOpts {

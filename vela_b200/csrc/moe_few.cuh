@@ -9,7 +9,7 @@
 namespace vela {
 namespace few {
 
-constexpr int WARPS = 16, TOKENS = 8, EXPERTS = 128, PAIRS = 32;
+constexpr int WARPS = 16, TOKENS = 8, EXPERTS = 128, PAIRS = 32;      // of few_up_kernel; what it can take
 constexpr int PART = 9;                   // floats from one expert's 8 partial scores to the next's
 
 constexpr int RANKS = 4;                  // blocks of a cluster, which share the scoring

@@ -167,9 +167,21 @@ template <class X, int FOLD, bool ZERO> __global__ void __cluster_dims__(few::RA
     float* part = reinterpret_cast<float*>(smem + few::stage_bytes<FOLD>(a.T, nu));
     const int mine = few::score_tiles(a.E) * 16;          // experts whose scores this block forms, at most
     few::part_scores<X>(x, a.ldx, a.T, static_cast<const X*>(a.router), a.E, a.D, part + warp * mine * few::PART, rank, warp, lane);
-    for (int i = warp; i < a.T * nu; i += few::WARPS) {
-        const int tok = w4::quot(i, nu), u = i - tok * nu;
-        w4::stage_unit<X, FOLD>(x + size_t(tok) * a.ldx + u * 128 + 4 * lane, a.D - u * 128 - 4 * lane, xs + size_t(i) * 128, xp + size_t(i) * (128 / FOLD), lane);
+    for (int i0 = warp; i0 < a.T * nu; i0 += 4 * few::WARPS) {     // four units under way at a time
+        uint2 raw[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + j * few::WARPS, tok = w4::quot(i, nu), c = (i - tok * nu) * 128 + 4 * lane;
+            raw[j] = i < a.T * nu && c < a.D ? __ldg(reinterpret_cast<const uint2*>(x + size_t(tok) * a.ldx + c)) : make_uint2(0u, 0u);      // D % 8 == 0
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + j * few::WARPS;
+            if (i >= a.T * nu) break;
+            const X* e = reinterpret_cast<const X*>(&raw[j]);
+            float v[4] = {Elem<X>::get(e[0]), Elem<X>::get(e[1]), Elem<X>::get(e[2]), Elem<X>::get(e[3])};
+            w4::stage_values<X, FOLD>(v, xs + size_t(i) * 128, xp + size_t(i) * (128 / FOLD), lane);
+        }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < mine * few::TOKENS; i += few::WARPS * 32) {
@@ -269,8 +281,8 @@ template <class X, int FOLD, bool ZERO> __global__ void __cluster_dims__(few::RA
     }
 }
 
-template <int FOLD, bool ZERO> __global__ void __launch_bounds__(few::WARPS * 32, 2) few_down_kernel(const MoeArgs a) {
-    __shared__ float s_sum[few::WARPS][16];
+template <int FOLD, bool ZERO, int WARPS> __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) few_down_kernel(const MoeArgs a) {
+    __shared__ float s_sum[WARPS][16];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rt = w4::row_tiles(a.down), nu = w4::units(a.down), items = a.T * rt, n = a.topk * nu, wide = nu * 128;
     const w4::Consts k = w4::consts<__nv_bfloat16>();
@@ -281,7 +293,7 @@ template <int FOLD, bool ZERO> __global__ void __launch_bounds__(few::WARPS * 32
         const int tok = w4::quot(it, rt), r = it - tok * rt;
         float acc[2] = {};
 #pragma unroll 1
-        for (int q = warp; q < n; q += few::WARPS) {
+        for (int q = warp; q < n; q += WARPS) {
             const int j = w4::quot(q, nu), u = q - j * nu, p = tok * a.topk + j;
             w4::Unit<FOLD, ZERO> w[1];
             w4::load_last(w[0], w4::row_ptr(a.down, size_t(__ldg(a.ids + p)) * rt + r, u, lane), a.down, u);
@@ -298,7 +310,7 @@ template <int FOLD, bool ZERO> __global__ void __launch_bounds__(few::WARPS * 32
         if (threadIdx.x < 16 && col < a.D) {
             float v = 0.f;
 #pragma unroll
-            for (int w = 0; w < few::WARPS; ++w) v += s_sum[w][threadIdx.x];
+            for (int w = 0; w < WARPS; ++w) v += s_sum[w][threadIdx.x];
             const size_t at = size_t(tok) * a.ldy + col;
             if (a.ytype == VELA_T_BF16) static_cast<__nv_bfloat16*>(a.Y)[at] = __float2bfloat16_rn(v);
             else static_cast<__half*>(a.Y)[at] = __float2half_rn(v);
@@ -477,28 +489,34 @@ template <class X, int FOLD, bool ZERO> void launch_few(cudaStream_t st, MoeArgs
     const size_t smem = few::up_bytes<FOLD>(a.T, w4::units(a.up), a.E);
     static std::atomic<int> ready[64];
     once_per_device(ready, [&] { VELA_CUDA(cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM)); });
-    // whole clusters; all of a block's items in one round if there are warps for it, since a round costs a memory latency
-    const int blocks = 2 * sm_count(), items = a.T * a.topk * w4::row_tiles(a.up), grid = std::min(ceil_div(items, few::RANKS), std::max(1, blocks / few::RANKS)) * few::RANKS;
+    // no more clusters than run at a time (71 of 2 x 148 blocks; the others would wait for a whole kernel); all of a block's items in one round if there are warps for it, since a
+    // round costs a memory latency
+    const int items = a.T * a.topk * w4::row_tiles(a.up);
+    const int grid = std::min(ceil_div(items, few::RANKS), clusters_per_device(reinterpret_cast<const void*>(up), few::RANKS, few::WARPS * 32, smem)) * few::RANKS;
     const int ks = std::max(1, std::min(w4::units(a.up), few::WARPS / ceil_div(items, grid)));
     a.split_up = w4::Split{ks, few::WARPS / ks, 1};
     up<<<grid, few::WARPS * 32, smem, st>>>(a);
+    // 32 warps on a row tile where there is one for an SM at most, so that each has half as many units one after another (E = 64, D = 2048: 18.6 -> 16.1 us a layer), else two blocks of 16
+    // (D = 4096, where 32 took 22.3 us against 20.8)
+    const int rows = a.T * w4::row_tiles(a.down), sms = sm_count();
+    const bool wide = rows <= sms && a.topk * w4::units(a.down) > 16;
     // brought up while the first is still running; it waits for it before it reads anything
     cudaLaunchAttribute at[1] = {};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(std::min(a.T * w4::row_tiles(a.down), blocks)); cfg.blockDim = dim3(few::WARPS * 32); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
-    VELA_CUDA(cudaLaunchKernelEx(&cfg, few_down_kernel<FOLD, ZERO>, a));
+    cfg.gridDim = dim3(std::min(rows, 2 * sms)); cfg.blockDim = dim3(wide ? 1024 : 512); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
+    VELA_CUDA(cudaLaunchKernelEx(&cfg, wide ? few_down_kernel<FOLD, ZERO, 32> : few_down_kernel<FOLD, ZERO, 16>, a));
 }
 template <int FOLD> void launch_few(cudaStream_t st, const MoeArgs& a) {
     if (a.ytype == VELA_T_BF16) a.up.zero ? launch_few<__nv_bfloat16, FOLD, true>(st, a) : launch_few<__nv_bfloat16, FOLD, false>(st, a);
     else a.up.zero ? launch_few<__half, FOLD, true>(st, a) : launch_few<__half, FOLD, false>(st, a);
 }
-// Which form.  Measured over 1 to 8 tokens, widths 512 to 4096, 8 to 128 experts of 256 to 2048 (units: gate and up units of 128 columns for each SM): the few-token form takes
-// 7.5 to 23 us against 16 to 26 of the other up to 64 units, loses above (T = 8, 129 units: 31 against 26), and with one token, where no weight is shared, still wins at 166 (27 against 30).
+// Which form.  Measured over 1 to 8 tokens, widths 512 to 4096, 8 to 128 experts of 256 to 2048, by the gate and up units of 128 columns for each SM and one and a half times the
+// units of the tokens' rows, which every block stages: the few-token form takes 7 to 24 us against 16 to 32 of the other up to 330, and 39 against 38 at 540, 36 against 28 at 490.
 template <int FOLD> bool is_few(const MoeArgs& a, int router_type) {
-    const double units = double(a.T) * a.topk * w4::row_tiles(a.up) * w4::units(a.up) / sm_count();
-    return units <= (a.T == 1 ? 192 : 64) && a.T <= few::TOKENS && a.E <= few::EXPERTS && a.T * a.topk <= few::PAIRS && router_type == a.ytype && a.vecx && a.vecr &&
+    const double units = double(a.T) * a.topk * w4::row_tiles(a.up) * w4::units(a.up) / sm_count() + 1.5 * a.T * w4::units(a.up);
+    return units <= 430 && a.T <= few::TOKENS && a.E <= few::EXPERTS && a.T * a.topk <= few::PAIRS && router_type == a.ytype && a.vecx && a.vecr &&
            size_t(a.E) * a.D <= FEW_ROUTER && few::up_bytes<FOLD>(a.T, w4::units(a.up), a.E) <= FEW_SMEM && !a.extra;
 }
 template <int FOLD> void launch(cudaStream_t st, MoeArgs a, int router_type) {

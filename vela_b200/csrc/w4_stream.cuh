@@ -67,12 +67,8 @@ template <int FOLD> __device__ __forceinline__ void load_staged(uint32_t (&b)[16
 #pragma unroll
     for (int f = 0; f < 128 / FOLD; ++f) { p.v[f][0] = __ldg(e + f); p.v[f][1] = __ldg(o + f); }
 }
-// Stages one unit of a row of X, a warp together: columns 4 lane .. 4 lane + 3 (n of them exist, from p on) to `out` (the unit's 128 values); the first lane of each fold writes its
-// pair {factor that the staged values have lost, their sum}.
-template <class X, int FOLD> __device__ __forceinline__ void stage_unit(const X* p, int n, __half* out, float2* pair, int lane) {
-    float v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? Elem<X>::get(p[i]) : 0.f;
+// What a warp has of a staged unit (stage_unit below).
+template <class X, int FOLD> __device__ __forceinline__ void stage_values(float (&v)[4], __half* out, float2* pair, int lane) {
     float2 s = make_float2(1.f, 1.f);
     if constexpr (Elem<X>::code != VELA_T_F16) {
         uint32_t top = 0;
@@ -87,6 +83,14 @@ template <class X, int FOLD> __device__ __forceinline__ void stage_unit(const X*
 #pragma unroll
     for (int o = 1; o < FOLD / 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane % (FOLD / 4) == 0) pair[lane / (FOLD / 4)] = make_float2(s.y, sum);
+}
+// Stages one unit of a row of X, a warp together: columns 4 lane .. 4 lane + 3 (n of them exist, from p on) to `out` (the unit's 128 values); the first lane of each fold writes its
+// pair {factor that the staged values have lost, their sum}.
+template <class X, int FOLD> __device__ __forceinline__ void stage_unit(const X* p, int n, __half* out, float2* pair, int lane) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? Elem<X>::get(p[i]) : 0.f;
+    stage_values<X, FOLD>(v, out, pair, lane);
 }
 // One unit of a row of floats (x as above) as the sum of two f16 values.  Plain loads: another block of the same kernel may have written them.  left is a multiple of 8, p aligned to 16 bytes.
 template <int FOLD> __device__ __forceinline__ void load_floats(uint32_t (&b)[32], Pairs<FOLD>& p, const float* x, int left, int t) {
