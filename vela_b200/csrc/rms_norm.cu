@@ -174,15 +174,14 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
     }
 }
 
-// A warp a row for short rows (without a block's meeting; up to 1024 columns only where there are rows enough to hide that each warp then takes 4 vectors one after another:
-// 77 rows of 1024 take 4.8 us so and 2.4 by blocks), else a block of as many threads as the row has pairs of vectors, so that few of them idle.
+// A warp a row where it has one vector for each lane (8192 x 256 bf16: 3.7 us against 6.1 with a block a row; with two for each lane 8192 x 512 takes 7.9 against 8.0, so those go by blocks).  Else a block of as
+// many threads as the row has vectors while those are few for the GPU (128 x 4096: 2.6 us against 2.7 with two vectors a thread), and as it has pairs of vectors otherwise
+// (256 x 4096: 3.1 against 3.2; 2048 x 4096: 14.2 against 17.0; four a thread: 15.7).  Four where two are not enough for 512 threads.
 template <class T, int QT, bool VEC> void launch(cudaStream_t st, const NormArgs& a) {
     const int nv = ceil_div(a.C, 8), warps = 8;
     auto block = [&](int v) { return ceil_div(ceil_div(nv, v), 32) * 32; };
     if (nv <= 32) rms_norm_kernel<T, QT, 1, true, VEC><<<ceil_div(a.M, warps), 32 * warps, 0, st>>>(a);
-    else if (nv <= 64) rms_norm_kernel<T, QT, 2, true, VEC><<<ceil_div(a.M, warps), 32 * warps, 0, st>>>(a);
-    else if (nv <= 128 && a.M >= 4096) rms_norm_kernel<T, QT, 4, true, VEC><<<ceil_div(a.M, warps), 32 * warps, 0, st>>>(a);
-    else if (nv <= 512 && a.M <= 128) rms_norm_kernel<T, QT, 1, false, VEC><<<a.M, block(1), 0, st>>>(a);
+    else if (nv <= 512 && (long long)a.M * nv <= 512 * sm_count()) rms_norm_kernel<T, QT, 1, false, VEC><<<a.M, block(1), 0, st>>>(a);
     else if (nv <= 1024) rms_norm_kernel<T, QT, 2, false, VEC><<<a.M, block(2), 0, st>>>(a);
     else if (nv <= 2048) rms_norm_kernel<T, QT, 4, false, VEC><<<a.M, block(4), 0, st>>>(a);
     else rms_norm_long_kernel<T, QT, 512><<<a.M, 512, 0, st>>>(a, VEC);
