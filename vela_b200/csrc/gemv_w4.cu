@@ -156,11 +156,14 @@ template <int XT, int NT, int R, int BLOCKS> void launch(cudaStream_t st, const 
         else launch<XT, NT, R, BLOCKS, 128, false>(st, a);
     }
 }
+// Rows of X at a time, and one or two row tiles to a warp.  Up to 8 rows take one column tile and two blocks on an SM.  Beyond that the tensor pipe bounds the kernel, and two row tiles share what is
+// read of X: 16x8192x8192 bf16 takes 13.2 us with them and 16.7 without, 32x8192x8192 (two passes over the weights, the second from L2) 22.6 and 27.5; four column tiles in one pass would take
+// 27.5 too.  Where there is no second row tile for each SM one is faster (16x2368x4096: 4.3 against 5.1 us).  17 to 24 rows: three column tiles 21.2 us at 24x8192x8192, two passes 22.3.
 template <int XT> void launch(cudaStream_t st, const GemvArgs& a) {
     if (a.M <= 8) launch<XT, 1, 1, 2>(st, a);
-    else if (a.M <= 16) launch<XT, 2, 2, 1>(st, a);
-    else if (a.M <= 24) launch<XT, 3, 1, 1>(st, a);
-    else launch<XT, 4, 1, 1>(st, a);
+    else if (a.M > 16 && a.M <= 24) launch<XT, 3, 1, 1>(st, a);
+    else if (w4::row_tiles(a.W) > sm_count()) launch<XT, 2, 2, 1>(st, a);
+    else launch<XT, 2, 1, 1>(st, a);
 }
 
 void gemv_w4(cudaStream_t st, int xtype, GemvArgs a, int xgroup) {
