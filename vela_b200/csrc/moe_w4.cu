@@ -6,7 +6,7 @@
 // Else: route_kernel, a cluster of 8 blocks for each token, scores the experts (a warp for each), chooses, and stages the token's row for the products (w4_stream.cuh); it also clears
 // the other kernel's counters.  expert_kernel, one block on each SM (a cooperative launch), does all chosen experts' gate and up products, then their down products, then the weighed
 // sums, with a barrier over the whole grid in between.  An item is one row tile of one expert, for all tokens that chose it (columns of one product, so weights are read once
-// for every 8 NT of them); a block takes a run of neighbouring items, so an expert's activations stay in its registers.  A barrier costs about 1.5 us, over which the next
+// for every 8 of them); a block takes a run of neighbouring items, so an expert's activations stay in its registers.  A barrier costs about 1.5 us, over which the next
 // weights are already on their way to the L2 cache.
 //   Up: a row tile is 8 gate rows and their 8 up rows, so one thread sums both parts of a hidden value, which is kept as a float.
 //   Down: the result of each token and expert by itself, as floats; then each output is summed over the token's experts in the order of their places.
@@ -31,6 +31,11 @@ constexpr int WARPS = w4::WARPS;          // of expert_kernel
 constexpr int FEW_SMEM = 96 * 1024;           // of two blocks on an SM
 constexpr size_t FEW_ROUTER = 512 * 1024;     // elements of the router that a cluster reads
 constexpr int COUNTERS = 2;               // one for each barrier
+constexpr int ROOM = 96;                  // columns times rounds whose sums expert_kernel's shared memory holds
+constexpr size_t ROOM_BYTES = w4::sum_bytes(1, ROOM);
+// Units of a row tile that a warp takes in the up phase: two share their sums' way to shared memory, but with four scales for each the registers spill
+// (32 tokens, 32 experts of 4096 x 1536: groups of 64 take 118 us with two and 122 with one, groups of 32 181 and 149).
+template <int FOLD> constexpr int UP_UNITS = FOLD >= 64 ? 2 : 1;
 static __device__ unsigned g_moe_err;
 
 struct MoeArgs {
@@ -46,7 +51,6 @@ struct MoeArgs {
     bool vecx, vecr;
     int t0, tn;                       // expert_kernel: its tokens
     w4::Split split_up, split_down;
-    int room, room_bytes;             // its shared memory for sums: columns times rounds
     unsigned* err; long long limit; unsigned extra;
 };
 
@@ -102,6 +106,7 @@ template <class X, class RW, int FOLD> __global__ void __cluster_dims__(RANKS, 1
     const int gw = rank * ROUTE_WARPS + warp;
     const X* x = static_cast<const X*>(a.X) + size_t(tok) * a.ldx;
     float* lead = cluster.map_shared_rank(p, 0);
+    cluster.sync();                                        // all have begun: their shared memory may be written
     for (int e = gw; e < a.E; e += RANKS * ROUTE_WARPS) {
         const float s = dot_row(x, static_cast<const RW*>(a.router) + size_t(e) * a.D, a.D, a.vecx, a.vecr, lane);
         if (lane == 0) lead[e] = s;
@@ -160,6 +165,7 @@ template <class X, int FOLD, bool ZERO> __global__ void __cluster_dims__(few::RA
     __shared__ float s_sum[few::WARPS][16];
     asm volatile("griddepcontrol.launch_dependents;");     // few_down_kernel may be brought up
     cg::cluster_group cluster = cg::this_cluster();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, nu = w4::units(a.up), rank = blockIdx.x % few::RANKS;
     const X* x = static_cast<const X*>(a.X);
     __half* xs = reinterpret_cast<__half*>(smem);
@@ -184,6 +190,7 @@ template <class X, int FOLD, bool ZERO> __global__ void __cluster_dims__(few::RA
         }
     }
     __syncthreads();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");       // all have begun: their shared memory may be written
     for (int i = threadIdx.x; i < mine * few::TOKENS; i += few::WARPS * 32) {
         const int at = i >> 3, tok = i & 7, e = (at / 16 * few::RANKS + rank) * 16 + at % 16;
         if (e >= a.E || tok >= a.T) continue;
@@ -286,7 +293,8 @@ template <int FOLD, bool ZERO, int WARPS> __global__ void __launch_bounds__(WARP
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rt = w4::row_tiles(a.down), nu = w4::units(a.down), items = a.T * rt, n = a.topk * nu, wide = nu * 128;
     const w4::Consts k = w4::consts<__nv_bfloat16>();
-    asm volatile("griddepcontrol.wait;" ::: "memory");     // few_up_kernel has ended and its results are visible
+    // few_up_kernel has ended and its results are visible; they were written while this kernel was already there, so all are read by plain loads
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     // the two terms of a hidden value are columns 0 and 1 of the product (and 2 to 7 again, which are not used)
     const __nv_bfloat16* h = (g & 1 ? a.lo : a.hi) + 8 * t;
     for (int it = blockIdx.x; it < items; it += gridDim.x) {
@@ -296,11 +304,11 @@ template <int FOLD, bool ZERO, int WARPS> __global__ void __launch_bounds__(WARP
         for (int q = warp; q < n; q += WARPS) {
             const int j = w4::quot(q, nu), u = q - j * nu, p = tok * a.topk + j;
             w4::Unit<FOLD, ZERO> w[1];
-            w4::load_last(w[0], w4::row_ptr(a.down, size_t(__ldg(a.ids + p)) * rt + r, u, lane), a.down, u);
+            w4::load_last(w[0], w4::row_ptr(a.down, size_t(a.ids[p]) * rt + r, u, lane), a.down, u);
             float c[1][1][4] = {};
             const __nv_bfloat16* x[1] = {h + size_t(p) * wide + u * 128};
-            w4::unit<VELA_T_BF16, true, 1, 1>(c, w, x, 0, a.down.f16, k, [](int, int) { return make_float2(1.f, 1.f); });
-            const float y = __ldg(a.weights + p);
+            w4::unit<VELA_T_BF16, true, 1, 1, false>(c, w, x, 0, a.down.f16, k, [](int, int) { return make_float2(1.f, 1.f); });
+            const float y = a.weights[p];
             acc[0] = fmaf(y, c[0][0][0] + c[0][0][1], acc[0]);
             acc[1] = fmaf(y, c[0][0][2] + c[0][0][3], acc[1]);
         }
@@ -337,15 +345,15 @@ __device__ __forceinline__ bool grid_barrier(unsigned* count, unsigned want, uns
     return *flag != 0;
 }
 
-template <int NT, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS * 32, 1) expert_kernel(const MoeArgs a) {
+template <int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS * 32, 1) expert_kernel(const MoeArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int s_n, s_flag;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int grid = gridDim.x, P = a.tn * a.topk, p0 = a.t0 * a.topk;
     float* sums = reinterpret_cast<float*>(smem);
-    int32_t* s_list = reinterpret_cast<int32_t*>(smem + a.room_bytes);
+    int32_t* s_list = reinterpret_cast<int32_t*>(smem + ROOM_BYTES);
     int32_t* s_ids = s_list + P;
-    int32_t* s_expert = s_ids + P;                  // slot v has expert s_expert[v] and the pairs (token * topk + place) s_at[s_first[v]] .. s_at[s_first[v + 1] - 1], 8 NT at most
+    int32_t* s_expert = s_ids + P;                  // slot v has expert s_expert[v] and the pairs (token * topk + place) s_at[s_first[v]] .. s_at[s_first[v + 1] - 1], 8 at most
     int32_t* s_first = s_expert + P;
     int32_t* s_cnt = s_first + P + 1;
     int32_t* s_at = s_cnt + a.E;
@@ -364,14 +372,14 @@ template <int NT, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS *
         }
         int n = 0, at = 0;                              // first places and slots, by expert; s_cnt becomes the first place
         for (int e0 = 0; e0 < a.E; e0 += 32) {
-            const int e = e0 + lane, c = e < a.E ? s_cnt[e] : 0, v = (c + 8 * NT - 1) / (8 * NT);
+            const int e = e0 + lane, c = e < a.E ? s_cnt[e] : 0, v = (c + 7) >> 3;
             if (__ballot_sync(0xffffffffu, c) == 0) continue;
             int ci = c, vi = v;
             for (int o = 1; o < 32; o <<= 1) {
                 const int x = __shfl_up_sync(0xffffffffu, ci, o), y = __shfl_up_sync(0xffffffffu, vi, o);
                 if (lane >= o) { ci += x; vi += y; }
             }
-            for (int i = 0; i < v; ++i) { s_expert[n + vi - v + i] = e; s_first[n + vi - v + i] = at + ci - c + i * 8 * NT; }
+            for (int i = 0; i < v; ++i) { s_expert[n + vi - v + i] = e; s_first[n + vi - v + i] = at + ci - c + 8 * i; }
             if (c) s_cnt[e] = at + ci - c;
             n += __shfl_sync(0xffffffffu, vi, 31);
             at += __shfl_sync(0xffffffffu, ci, 31);
@@ -405,10 +413,10 @@ template <int NT, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS *
 
     ask(a.up, share(w4::row_tiles(a.up), blockIdx.x), share(w4::row_tiles(a.up), blockIdx.x + 1));
     runs(a.up, [&](int v, size_t tile0, int r0, int r1, int c) {
-        const int nu = w4::units(a.up), room = w4::quot(a.room, c);
-        w4::stream<w4::F, NT, NT == 1 && FOLD == 128 ? 2 : 1, FOLD, ZERO, true>(a.up, tile0, r0, r1, c, a.split_up, sums, room,
-            [&](int n, int u, uint32_t (&b)[16], w4::Pairs<FOLD>& p) {
-                auto at = [&](int col) { return size_t(a.t0 + s_tok[s_first[v] + min(8 * n + col, c - 1)]) * nu + u; };     // any row where there is none: its column is not used
+        const int nu = w4::units(a.up), room = w4::quot(ROOM, c);
+        w4::stream<w4::F, UP_UNITS<FOLD>, FOLD, ZERO, true>(a.up, tile0, r0, r1, c, a.split_up, sums, room,
+            [&](int u, uint32_t (&b)[16], w4::Pairs<FOLD>& p) {
+                auto at = [&](int col) { return size_t(a.t0 + s_tok[s_first[v] + min(col, c - 1)]) * nu + u; };     // any row where there is none: its column is not used
                 w4::load_staged<FOLD>(b, p, a.xs + at(g) * 128 + 8 * t, a.xp + at(2 * t) * (128 / FOLD), a.xp + at(2 * t + 1) * (128 / FOLD));
             },
             [&](int rt, int col, int i, float gate, float up) { a.h[size_t(pair_of(v, col)) * a.I + rt * 8 + i] = gate / (1.f + expf(-gate)) * up; });
@@ -419,9 +427,9 @@ template <int NT, int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS *
 
     const int wide = w4::row_tiles(a.down) * 16;
     runs(a.down, [&](int v, size_t tile0, int r0, int r1, int c) {
-        w4::stream<w4::H, NT, 1, FOLD, ZERO, false>(a.down, tile0, r0, r1, c, a.split_down, sums, w4::quot(a.room, c),
-            [&](int n, int u, uint32_t (&b)[32], w4::Pairs<FOLD>& p) {
-                w4::load_floats<FOLD>(b, p, a.h + size_t(pair_of(v, min(8 * n + g, c - 1))) * a.I + u * 128 + 8 * t, a.I - u * 128 - 8 * t, t);
+        w4::stream<w4::H, 1, FOLD, ZERO, false>(a.down, tile0, r0, r1, c, a.split_down, sums, w4::quot(ROOM, c),
+            [&](int u, uint32_t (&b)[32], w4::Pairs<FOLD>& p) {
+                w4::load_floats<FOLD>(b, p, a.h + size_t(pair_of(v, min(g, c - 1))) * a.I + u * 128 + 8 * t, a.I - u * 128 - 8 * t, t);
             },
             [&](int rt, int col, int row, float y, float) { a.o[size_t(pair_of(v, col)) * wide + rt * 16 + row] = y; });
     });
@@ -466,19 +474,16 @@ void check(const vela_moe& L, int T) {
     VELA_REQUIRE((L.gate_up.zero != nullptr) == (L.down.zero != nullptr), "moe_w4: gate_up and down both have zero points or neither");
 }
 
-template <int NT, int FOLD, bool ZERO> void launch_experts(cudaStream_t st, MoeArgs a) {
-    auto* kernel = expert_kernel<NT, FOLD, ZERO>;
+template <int FOLD, bool ZERO> void launch_experts(cudaStream_t st, MoeArgs a) {
+    auto* kernel = expert_kernel<FOLD, ZERO>;
     // as many experts as the tokens reach on average
     const int grid = sm_count();
     const double slots = a.E * (1 - std::pow(1 - double(a.topk) / a.E, a.tn));
     auto run = [&](const w4::Weights& W) { return std::min(w4::row_tiles(W), std::max(1, int(slots * w4::row_tiles(W) / grid))); };
-    a.split_up = w4::plan(w4::units(a.up), NT == 1 && FOLD == 128 ? 2 : 1, run(a.up));
+    a.split_up = w4::plan(w4::units(a.up), UP_UNITS<FOLD>, run(a.up));
     a.split_down = w4::plan(w4::units(a.down), 1, run(a.down));
-    // room for the sums of so many columns times rounds, then the slots
-    a.room = NT == 1 ? 96 : 48;
-    a.room_bytes = int(w4::sum_bytes(1, a.room));
-    const size_t smem = a.room_bytes + (size_t(a.tn) * a.topk * 6 + 1 + a.E) * 4;
-    constexpr size_t most = w4::sum_bytes(1, 96) + (size_t(T_BLOCK) * K_MAX * 6 + 1 + E_MAX) * 4;
+    const size_t smem = ROOM_BYTES + (size_t(a.tn) * a.topk * 6 + 1 + a.E) * 4;
+    constexpr size_t most = ROOM_BYTES + (size_t(T_BLOCK) * K_MAX * 6 + 1 + E_MAX) * 4;
     static std::atomic<int> ready[64];
     once_per_device(ready, [&] { VELA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most))); });
     void* args[] = {&a};
@@ -532,10 +537,7 @@ template <int FOLD> void launch(cudaStream_t st, MoeArgs a, int router_type) {
     }
     for (a.t0 = 0; a.t0 < a.T; a.t0 += T_BLOCK) {
         a.tn = std::min(T_BLOCK, a.T - a.t0);
-        // 16 columns at a time where an expert has more than 8 tokens as a rule (its weights are then read once), else 8
-        const bool one = a.tn <= 8 || a.tn * a.topk <= 6 * a.E;
-        if (a.up.zero) one ? launch_experts<1, FOLD, true>(st, a) : launch_experts<2, FOLD, true>(st, a);
-        else one ? launch_experts<1, FOLD, false>(st, a) : launch_experts<2, FOLD, false>(st, a);
+        a.up.zero ? launch_experts<FOLD, true>(st, a) : launch_experts<FOLD, false>(st, a);
     }
 }
 

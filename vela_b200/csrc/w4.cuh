@@ -154,11 +154,12 @@ template <> struct Act<VELA_T_E4M3> { typedef uint8_t X; typedef __half M; stati
 template <> struct Act<VELA_T_I8> { typedef uint8_t X; typedef int8_t M; static constexpr bool scaled = true, integer = true; static constexpr int REGS = 2; };
 
 // A lane's 8 activations p[0 .. 8) of a 32-column part as operands.  Not WHOLE: n of them exist (may be negative), zeros stand for the others,
-// and p has its type's alignment only.
-template <int XT, bool WHOLE> __device__ __forceinline__ void load_x8(uint32_t (&b)[Act<XT>::REGS], const typename Act<XT>::X* p, int n) {
+// and p has its type's alignment only.  CONSTANT: nobody writes them while the kernel is there.
+template <int XT, bool WHOLE, bool CONSTANT = true> __device__ __forceinline__ void load_x8(uint32_t (&b)[Act<XT>::REGS], const typename Act<XT>::X* p, int n) {
+    static_assert(CONSTANT || sizeof(typename Act<XT>::X) == 2, "8-bit rows are always read as constants");
     if constexpr (sizeof(typename Act<XT>::X) == 2) {
         if constexpr (WHOLE) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+            const uint4 u = CONSTANT ? __ldg(reinterpret_cast<const uint4*>(p)) : *reinterpret_cast<const uint4*>(p);
             b[0] = u.x; b[1] = u.y; b[2] = u.z; b[3] = u.w;
         } else {
             const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
@@ -192,7 +193,7 @@ template <int XT, bool WHOLE> __device__ __forceinline__ void load_x8(uint32_t (
 // Adds one unit of R row tiles to acc: c0, c1 = row g and activation rows 2t, 2t + 1; c2, c3 = row g + 8.  x[n]: this lane's place (row g of column
 // tile n, column 8 t of the unit; any row where there is none: its column of the product is not used); WHOLE: all 128 columns exist and x is aligned
 // to 8 of them, else left columns exist from x on; sx(f, n): the scales of activation rows 2t, 2t + 1 of column tile n in fold f (8-bit forms).
-template <int XT, bool WHOLE, int NT, int R, int FOLD, bool ZERO, class SX>
+template <int XT, bool WHOLE, int NT, int R, bool CONSTANT = true, int FOLD, bool ZERO, class SX>
 __device__ __forceinline__ void unit(float (&acc)[R][NT][4], const Unit<FOLD, ZERO> (&W)[R], const typename Act<XT>::X* const (&x)[NT], int left, bool f16,
                                      const Consts& k, SX sx) {
     typedef typename Act<XT>::M M;
@@ -201,7 +202,7 @@ __device__ __forceinline__ void unit(float (&acc)[R][NT][4], const Unit<FOLD, ZE
     uint32_t all[AHEAD ? 4 : 1][NT][Act<XT>::REGS];
     if constexpr (AHEAD) {
 #pragma unroll
-        for (int h = 0; h < 4; ++h) load_x8<XT, WHOLE>(all[h][0], x[0] + 32 * h, left - 32 * h);
+        for (int h = 0; h < 4; ++h) load_x8<XT, WHOLE, CONSTANT>(all[h][0], x[0] + 32 * h, left - 32 * h);
     }
 #pragma unroll
     for (int f = 0; f < 128 / FOLD; ++f) {
@@ -215,7 +216,7 @@ __device__ __forceinline__ void unit(float (&acc)[R][NT][4], const Unit<FOLD, ZE
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     if constexpr (AHEAD) { b[n][0] = all[h][n][0]; b[n][1] = all[h][n][1]; }
-                    else load_x8<XT, WHOLE>(b[n], x[n] + 32 * h, left - 32 * h);
+                    else load_x8<XT, WHOLE, CONSTANT>(b[n], x[n] + 32 * h, left - 32 * h);
                     mma_i8(s[n], 0x01010101u, 0u, 0x01010101u, 0u, b[n][0], b[n][1]);
                 }
 #pragma unroll
@@ -255,7 +256,7 @@ __device__ __forceinline__ void unit(float (&acc)[R][NT][4], const Unit<FOLD, ZE
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     if constexpr (AHEAD) { b[n][0] = all[h][n][0]; b[n][1] = all[h][n][1]; b[n][2] = all[h][n][2]; b[n][3] = all[h][n][3]; }
-                    else load_x8<XT, WHOLE>(b[n], x[n] + 32 * h, left - 32 * h);
+                    else load_x8<XT, WHOLE, CONSTANT>(b[n], x[n] + 32 * h, left - 32 * h);
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j)

@@ -146,7 +146,6 @@ __device__ __forceinline__ void multiply(float (&acc)[4], const Unit<FOLD, ZERO>
 // ---------------------------------------------------------------- streaming row tiles past stationary activations
 constexpr int WARPS = 16;                 // of a block; one block on each SM
 constexpr int COL = 20;                   // floats from one column's 16 sums to the next: stores are free of bank conflicts
-constexpr size_t SUMS = 160 * 1024;       // bytes of shared memory for sums, at most
 __host__ __device__ constexpr size_t sum_bytes(int cols, int rounds) { return size_t(WARPS) * cols * COL * 4 * rounds; }
 
 // How a block splits a product: ks warps share out the units of a row tile, UW to each at a time (a chunk; several where there are more), and the block takes slots = WARPS / ks
@@ -163,11 +162,11 @@ inline Split plan(int nu, int uw, int nrow) {
     return best;
 }
 
-// The block's share: row tiles r0 .. r1 - 1 (at least one) of a matrix whose first row tile is number tile0, against `cols` <= 8 NT activation rows.
+// The block's share: row tiles r0 .. r1 - 1 (at least one) of a matrix whose first row tile is number tile0, against `cols` <= 8 activation rows.
 // Weights are loaded one round ahead.  A warp's sums go to shared memory and are added there, in the order of the warps, once for `room`
-// rounds (sum_bytes).  load(n, u, b, pairs): operands of column tile n, unit u, by a whole warp; out(rt, col, row or half row, sums):
+// rounds (sum_bytes).  load(u, b, pairs): operands of unit u, by a whole warp; out(rt, col, row or half row, sums):
 // called by one thread for each row of 16, or with PAIRED for each i < 8 with the sums of rows i and i + 8.
-template <Kind KIND, int NT, int UW, int FOLD, bool ZERO, bool PAIRED, class LOAD, class OUT>
+template <Kind KIND, int UW, int FOLD, bool ZERO, bool PAIRED, class LOAD, class OUT>
 __device__ __forceinline__ void stream(const Weights& W, size_t tile0, int r0, int r1, int cols, const Split& split, float* sums, int room, LOAD load, OUT out) {
     typedef Unit<FOLD, ZERO> U;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -214,8 +213,8 @@ __device__ __forceinline__ void stream(const Weights& W, size_t tile0, int r0, i
         fq += qstep; fs += sstep;
         if constexpr (ZERO) fz += sstep;
     };
-    uint32_t b[UW][NT][regs<KIND>()];
-    Pairs<FOLD> p[UW][NT];
+    uint32_t b[UW][regs<KIND>()];
+    Pairs<FOLD> p[UW];
     U one[UW], two[UW];
     seek(0, 0);
     if (count(0, most) > 0) fetch(one);
@@ -224,18 +223,16 @@ __device__ __forceinline__ void stream(const Weights& W, size_t tile0, int r0, i
         for (int c = 0; c < chunks; ++c) {
             if (chunks > 1 || base == 0) {
 #pragma unroll
-                for (int i = 0; i < UW; ++i)
+                for (int i = 0; i < UW; ++i) {
+                    const int u = (c * ks + kw) * UW + i;
+                    load(min(u, nu - 1), b[i], p[i]);
+                    if (u >= nu) {
 #pragma unroll
-                    for (int m = 0; m < NT; ++m) {
-                        const int u = (c * ks + kw) * UW + i;
-                        load(m, min(u, nu - 1), b[i][m], p[i][m]);
-                        if (u >= nu) {
+                        for (int r = 0; r < regs<KIND>(); ++r) b[i][r] = 0u;
 #pragma unroll
-                            for (int r = 0; r < regs<KIND>(); ++r) b[i][m][r] = 0u;
-#pragma unroll
-                            for (int f = 0; f < 128 / FOLD; ++f) p[i][m].v[f][0] = p[i][m].v[f][1] = make_float2(0.f, 0.f);
-                        }
+                        for (int f = 0; f < 128 / FOLD; ++f) p[i].v[f][0] = p[i].v[f][1] = make_float2(0.f, 0.f);
                     }
+                }
             }
             if (c > 0 || base > 0) {                        // what was fetched at the end of the last chunk
 #pragma unroll
@@ -243,20 +240,16 @@ __device__ __forceinline__ void stream(const Weights& W, size_t tile0, int r0, i
             }
             float* d = mine + 2 * t * COL + g;
             auto work = [&](const U (&w)[UW]) {
-                float acc[NT][4] = {};
+                float acc[4] = {};
 #pragma unroll
-                for (int i = 0; i < UW; ++i)
+                for (int i = 0; i < UW; ++i) multiply<KIND, FOLD, ZERO>(acc, w[i], b[i], p[i], W.f16);
 #pragma unroll
-                    for (int m = 0; m < NT; ++m) multiply<KIND, FOLD, ZERO>(acc[m], w[i], b[i][m], p[i][m], W.f16);
-#pragma unroll
-                for (int m = 0; m < NT; ++m)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        if (8 * m + 2 * t + i < cols) {
-                            float* q = d + (8 * m + i) * COL;
-                            if (c) { acc[m][i] += q[0]; acc[m][i + 2] += q[8]; }
-                            q[0] = acc[m][i]; q[8] = acc[m][i + 2];
-                        }
+                for (int i = 0; i < 2; ++i)
+                    if (2 * t + i < cols) {
+                        float* q = d + i * COL;
+                        if (c) { acc[i] += q[0]; acc[i + 2] += q[8]; }
+                        q[0] = acc[i]; q[8] = acc[i + 2];
+                    }
                 d += cols * COL;
             };
             int j = 0;
