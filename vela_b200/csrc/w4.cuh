@@ -77,7 +77,8 @@ template <class M> __device__ __forceinline__ Consts consts() {
 }
 template <> __device__ __forceinline__ Consts consts<int8_t>() { return Consts{}; }
 
-// a / b for a >= 0, b > 0: the quotient of floats is off by a few at most, which the loops put right (a division of integers takes many times as long)
+// a / b for a >= 0, b > 0: the quotient of floats is off by a few at most, which the loops put right (a division of integers takes many
+// times as long)
 __device__ __forceinline__ int quot(int a, int b) {
     int q = int(__fdividef(float(a), float(b))), r = a - q * b;
     while (r < 0) { --q; r += b; }
@@ -99,7 +100,8 @@ __device__ __forceinline__ uint4 load_tile(const uint4* p) {
 }
 
 // A unit is two neighbouring tiles (128 columns) of one row tile: what a warp loads at once.  FOLD (32, 64 or 128) is the
-// number of columns between scalings, the smaller of the weights' and the activations' group; a unit has one scale (and zero) for each fold.
+// number of columns between scalings, the smaller of the weights' and the activations' group; a unit has one scale (and zero) for each
+// fold.
 template <int FOLD, bool ZERO> struct Unit {
     uint4 w[2];
     uint32_t s[128 / FOLD];
@@ -153,7 +155,8 @@ template <> struct Act<VELA_T_F16> { typedef __half X; typedef __half M; static 
 template <> struct Act<VELA_T_E4M3> { typedef uint8_t X; typedef __half M; static constexpr bool scaled = true, integer = false; static constexpr int REGS = 4; };
 template <> struct Act<VELA_T_I8> { typedef uint8_t X; typedef int8_t M; static constexpr bool scaled = true, integer = true; static constexpr int REGS = 2; };
 
-// A lane's 8 activations p[0 .. 8) of a 32-column part as operands.  Not WHOLE: n of them exist (may be negative), zeros stand for the others,
+// A lane's 8 activations p[0 .. 8) of a 32-column part as operands.  Not WHOLE: n of them exist (may be negative), zeros stand for the
+// others,
 // and p has its type's alignment only.  CONSTANT: nobody writes them while the kernel is there.
 template <int XT, bool WHOLE, bool CONSTANT = true> __device__ __forceinline__ void load_x8(uint32_t (&b)[Act<XT>::REGS], const typename Act<XT>::X* p, int n) {
     static_assert(CONSTANT || sizeof(typename Act<XT>::X) == 2, "8-bit rows are always read as constants");
@@ -190,9 +193,12 @@ template <int XT, bool WHOLE, bool CONSTANT = true> __device__ __forceinline__ v
     }
 }
 
-// Adds one unit of R row tiles to acc: c0, c1 = row g and activation rows 2t, 2t + 1; c2, c3 = row g + 8.  x[n]: this lane's place (row g of column
-// tile n, column 8 t of the unit; any row where there is none: its column of the product is not used); WHOLE: all 128 columns exist and x is aligned
-// to 8 of them, else left columns exist from x on; sx(f, n): the scales of activation rows 2t, 2t + 1 of column tile n in fold f (8-bit forms).
+// Adds one unit of R row tiles to acc: c0, c1 = row g and activation rows 2t, 2t + 1; c2, c3 = row g + 8.  x[n]: this lane's place (row
+// g of column
+// tile n, column 8 t of the unit; any row where there is none: its column of the product is not used); WHOLE: all 128 columns exist and
+// x is aligned
+// to 8 of them, else left columns exist from x on; sx(f, n): the scales of activation rows 2t, 2t + 1 of column tile n in fold f (8-bit
+// forms).
 template <int XT, bool WHOLE, int NT, int R, bool CONSTANT = true, int FOLD, bool ZERO, class SX>
 __device__ __forceinline__ void unit(float (&acc)[R][NT][4], const Unit<FOLD, ZERO> (&W)[R], const typename Act<XT>::X* const (&x)[NT], int left, bool f16,
                                      const Consts& k, SX sx) {
