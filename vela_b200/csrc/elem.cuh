@@ -44,6 +44,33 @@ template <class T> __device__ __forceinline__ void load_raw(Raw8<T>& x, const T*
         for (int i = 0; i < 8; ++i) if (i < n) x.e[i] = p[i];
     }
 }
+// A warp's 256 neighbouring elements (as bits E) in rows that have their type's alignment only: lane l loads and stores elements l, l + 32, ..., so that a warp's
+// 32 lie side by side; `line` (256 elements, the warp's own) brings them into the lanes' order, 8 neighbours each, and back.
+// p: the warp's first element; n: the elements that exist from there on (any number).
+template <class E> union Line8 { uint4 u[(sizeof(E) + 1) / 2]; uint2 h; uint32_t w[2 * sizeof(E)]; E e[8]; };
+template <class E> __device__ __forceinline__ void line_load(Line8<E>& x, const E* p, int n, int lane) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x.e[k] = 32 * k + lane < n ? p[32 * k + lane] : E(0);
+}
+template <class E> __device__ __forceinline__ void line_to_lanes(Line8<E>& x, E* line, int lane) {
+    static_assert(sizeof(E) >= 2, "16-byte loads");
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) line[32 * k + lane] = x.e[k];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < int(sizeof(E) / 2); ++i) x.u[i] = reinterpret_cast<const uint4*>(line + 8 * lane)[i];
+}
+template <class E> __device__ __forceinline__ void line_store(const Line8<E>& x, E* p, int n, E* line, int lane) {
+    __syncwarp();
+    if constexpr (sizeof(E) == 1) *reinterpret_cast<uint2*>(line + 8 * lane) = x.h;
+    else
+#pragma unroll
+        for (int i = 0; i < int(sizeof(E) / 2); ++i) reinterpret_cast<uint4*>(line + 8 * lane)[i] = x.u[i];
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) if (32 * k + lane < n) p[32 * k + lane] = line[32 * k + lane];
+}
 // x as floats
 template <class T> __device__ __forceinline__ void unpack8(float (&v)[8], const Raw8<T>& x) {
     if constexpr (Elem<T>::code == VELA_T_BF16) {
@@ -80,6 +107,8 @@ template <class T> __device__ __forceinline__ void pack8(Raw8<T>& x, const float
         for (int i = 0; i < 8; ++i) x.e[i] = Elem<T>::put(v[i]);
     }
 }
+template <class T> struct Bits { typedef uint16_t E; };
+template <> struct Bits<float> { typedef uint32_t E; };
 template <class T> __device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
     Raw8<T> x;
     pack8(x, v);

@@ -34,8 +34,9 @@ struct Sum { __device__ __forceinline__ float operator()(float a, float b) const
 struct Max { __device__ __forceinline__ float operator()(float a, float b) const { return max_nan(a, b); } };
 
 // 8 values of q = y * inv as bytes
-template <int QT> __device__ __forceinline__ void store_q8(uint8_t* p, int n, bool vec, const float (&y)[8], float inv) {
-    union { uint2 u; uint8_t b[8]; __nv_fp8x2_storage_t h[4]; } o;
+union Bytes8 { uint32_t w[2]; uint8_t b[8]; __nv_fp8x2_storage_t h[4]; };
+template <int QT> __device__ __forceinline__ Bytes8 quant8(const float (&y)[8], float inv) {
+    Bytes8 o;
     if constexpr (QT == VELA_T_I8) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) o.b[i] = uint8_t(max(-127, min(127, __float2int_rn(y[i] * inv))));
@@ -43,17 +44,23 @@ template <int QT> __device__ __forceinline__ void store_q8(uint8_t* p, int n, bo
 #pragma unroll
         for (int i = 0; i < 4; ++i) o.h[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i] * inv, y[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
     }
-    if (vec) *reinterpret_cast<uint2*>(p) = o.u;
+    return o;
+}
+__device__ __forceinline__ void store_q8(uint8_t* p, int n, bool vec, const Bytes8& o) {
+    if (vec) *reinterpret_cast<uint2*>(p) = make_uint2(o.w[0], o.w[1]);
     else
 #pragma unroll
         for (int i = 0; i < 8; ++i) if (i < n) p[i] = o.b[i];
 }
 
-// A block, or with WARP a warp, for each row; thread i holds values 8 (i + j n) .. + 7, j < V, in registers, n the row's threads.  All
-// three inputs are fetched
-// before the first reduction.  The group of 64 or 128 columns is 8 or 16 neighbouring lanes.  VEC: rows are whole and aligned vectors.
+// A block, or with WARP a warp, for each row; thread i holds values 8 (i + j n) .. + 7, j < V, in registers, n the row's threads.  All three
+// inputs are fetched before the first reduction.  The group of 64 or 128 columns is 8 or 16 neighbouring lanes.  VEC: rows are whole and
+// aligned vectors; others are loaded and stored with a warp's 32 elements side by side and brought into the lanes' order in shared memory
+// (elem.cuh): 8192 x 4095 bf16 takes 80 us so, 131 with each lane on its own 8 elements (and 126 by aligned blocks shifted into place).
 template <class T, int QT, int V, bool WARP, bool VEC> __global__ void __launch_bounds__(WARP ? 256 : 512) rms_norm_kernel(const NormArgs a) {
     __shared__ float red[2][16];
+    typedef typename Bits<T>::E E;
+    __shared__ __align__(16) E lines[VEC ? 1 : WARP ? 8 : 16][VEC ? 1 : 256];
     constexpr float TOP = QT == VELA_T_I8 ? 127.f : 448.f;
     const int n = WARP ? 32 : blockDim.x, ti = WARP ? threadIdx.x & 31 : threadIdx.x;
     const size_t row = WARP ? size_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
@@ -62,16 +69,39 @@ template <class T, int QT, int V, bool WARP, bool VEC> __global__ void __launch_
     const T* r = static_cast<const T*>(a.R) + row * a.ldr;
     const T* g = static_cast<const T*>(a.g);
     Raw8<T> rx[V], rr[V], rg[V];
+    const int lane = threadIdx.x & 31;
+    E* const line = lines[VEC ? 0 : threadIdx.x >> 5];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = 8 * (ti + j * n), left = a.C - c;
-        if (left <= 0) { load_raw(rx[j], x, 0, false); load_raw(rr[j], x, 0, false); load_raw(rg[j], g, 0, false); continue; }
-        load_raw(rx[j], x + c, left, VEC);
-        if (a.R) load_raw(rr[j], r + c, left, VEC);
-        load_raw(rg[j], g + c, left, VEC);
+        const int c = 8 * (ti + j * n), left = a.C - c, c0 = c - 8 * lane;
+        if (VEC && left <= 0) { load_raw(rx[j], x, 0, false); load_raw(rr[j], x, 0, false); load_raw(rg[j], g, 0, false); continue; }
+        if constexpr (VEC) {
+            load_raw(rx[j], x + c, left, true);
+            if (a.R) load_raw(rr[j], r + c, left, true);
+            load_raw(rg[j], g + c, left, true);
+        } else {
+            line_load(*reinterpret_cast<Line8<E>*>(&rx[j]), reinterpret_cast<const E*>(x + c0), a.C - c0, lane);
+            if (a.R) line_load(*reinterpret_cast<Line8<E>*>(&rr[j]), reinterpret_cast<const E*>(r + c0), a.C - c0, lane);
+            line_load(*reinterpret_cast<Line8<E>*>(&rg[j]), reinterpret_cast<const E*>(g + c0), a.C - c0, lane);
+        }
+    }
+    if constexpr (!VEC) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            line_to_lanes(*reinterpret_cast<Line8<E>*>(&rx[j]), line, lane);
+            if (a.R) line_to_lanes(*reinterpret_cast<Line8<E>*>(&rr[j]), line, lane);
+            line_to_lanes(*reinterpret_cast<Line8<E>*>(&rg[j]), line, lane);
+        }
     }
     float h[V][8];
     float ss = 0.f;
+    auto store = [&](T* p, int left, const float (&v)[8]) {
+        if constexpr (!VEC) {
+            Raw8<T> b;
+            pack8(b, v);
+            line_store(*reinterpret_cast<const Line8<E>*>(&b), reinterpret_cast<E*>(p - 8 * lane), left + 8 * lane, line, lane);
+        } else if (left > 0) store8(p, left, true, v);
+    };
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int c = 8 * (ti + j * n);
@@ -84,7 +114,7 @@ template <class T, int QT, int V, bool WARP, bool VEC> __global__ void __launch_
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(h[j][i], h[j][i], ss);
-        if (a.S && c < a.C) store8(static_cast<T*>(a.S) + row * a.lds + c, a.C - c, VEC, h[j]);
+        if (a.S) store(static_cast<T*>(a.S) + row * a.lds + c, a.C - c, h[j]);
     }
     const float rstd = rsqrtf(reduce<WARP>(ss, red[0], Sum()) / float(a.C) + a.eps);
     float top = 0.f, am[V];
@@ -97,7 +127,7 @@ template <class T, int QT, int V, bool WARP, bool VEC> __global__ void __launch_
 #pragma unroll
         for (int i = 0; i < 8; ++i) { h[j][i] = h[j][i] * rstd * t[i]; if (VEC || c + i < a.C) am[j] = max_nan(am[j], fabsf(h[j][i])); }
         if (VEC && c >= a.C) am[j] = 0.f;
-        if (a.Y && c < a.C) store8(static_cast<T*>(a.Y) + row * a.ldy + c, a.C - c, VEC, h[j]);
+        if (a.Y) store(static_cast<T*>(a.Y) + row * a.ldy + c, a.C - c, h[j]);
         top = max_nan(top, am[j]);
     }
     if (!a.Q) return;
@@ -111,10 +141,15 @@ template <class T, int QT, int V, bool WARP, bool VEC> __global__ void __launch_
             for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
             if (a.gshift == 7) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 8));
         }
-        if (c >= a.C) continue;
         m = m < AMAX_MIN ? AMAX_MIN : m;
-        if ((c & a.gmask) == 0) a.qscale[row * a.ngroups + (c >> a.gshift)] = m * (1.f / TOP);
-        store_q8<QT>(static_cast<uint8_t*>(a.Q) + row * a.ldq + c, a.C - c, VEC, h[j], TOP / m);
+        if (c < a.C && (c & a.gmask) == 0) a.qscale[row * a.ngroups + (c >> a.gshift)] = m * (1.f / TOP);
+        const Bytes8 q = quant8<QT>(h[j], TOP / m);
+        uint8_t* p = static_cast<uint8_t*>(a.Q) + row * a.ldq + c;
+        if constexpr (!VEC) {
+            Line8<uint8_t> b;
+            b.h = make_uint2(q.w[0], q.w[1]);
+            line_store(b, p - 8 * lane, a.C - c + 8 * lane, reinterpret_cast<uint8_t*>(line), lane);
+        } else if (c < a.C) store_q8(p, a.C - c, true, q);
     }
 }
 
@@ -173,7 +208,7 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
         if (n <= 0) continue;
         m = m < AMAX_MIN ? AMAX_MIN : m;
         if ((c & a.gmask) == 0) a.qscale[row * a.ngroups + (c >> a.gshift)] = m * (1.f / TOP);
-        store_q8<QT>(static_cast<uint8_t*>(a.Q) + row * a.ldq + c, n, vec, h, TOP / m);
+        store_q8(static_cast<uint8_t*>(a.Q) + row * a.ldq + c, n, vec, quant8<QT>(h, TOP / m));
     }
 }
 
