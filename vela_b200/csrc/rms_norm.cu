@@ -57,10 +57,13 @@ __device__ __forceinline__ void store_q8(uint8_t* p, int n, bool vec, const Byte
 // inputs are fetched before the first reduction.  The group of 64 or 128 columns is 8 or 16 neighbouring lanes.  VEC: rows are whole and
 // aligned vectors; others are loaded and stored with a warp's 32 elements side by side and brought into the lanes' order in shared memory
 // (elem.cuh): 8192 x 4095 bf16 takes 80 us so, 131 with each lane on its own 8 elements (and 126 by aligned blocks shifted into place).
-template <class T, int QT, int V, bool WARP, bool VEC> __global__ void __launch_bounds__(WARP ? 256 : 512) rms_norm_kernel(const NormArgs a) {
-    __shared__ float red[2][16];
+// threads; without alignment a block of 1024 is better than four vectors a thread, whose 107 registers leave room for one block
+// (2000 x 10241 f16: 79 us against 103), with it the smaller bound is (8192 x 4096 bf16: 39.5 against 40.5)
+template <class T, int V, bool WARP, bool VEC> constexpr int MOST = WARP ? 256 : V == 2 && sizeof(T) == 2 && !VEC ? 1024 : 512;
+template <class T, int QT, int V, bool WARP, bool VEC> __global__ void __launch_bounds__(MOST<T, V, WARP, VEC>) rms_norm_kernel(const NormArgs a) {
+    __shared__ float red[2][MOST<T, V, WARP, VEC> / 32];
     typedef typename Bits<T>::E E;
-    __shared__ __align__(16) E lines[VEC ? 1 : WARP ? 8 : 16][VEC ? 1 : 256];
+    __shared__ __align__(16) E lines[VEC ? 1 : MOST<T, V, WARP, VEC> / 32][VEC ? 1 : 256];
     constexpr float TOP = QT == VELA_T_I8 ? 127.f : 448.f;
     const int n = WARP ? 32 : blockDim.x, ti = WARP ? threadIdx.x & 31 : threadIdx.x;
     const size_t row = WARP ? size_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
@@ -213,18 +216,22 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
 }
 
 // A warp a row where it has one vector for each lane (8192 x 256 bf16: 3.7 us against 6.1 with a block a row; with two for each lane
-// 8192 x 512 takes 7.9 against 8.0, so those go by blocks).  Else a block of as
-// many threads as the row has vectors while those are few for the GPU (128 x 4096: 2.6 us against 2.7 with two vectors a thread), and
-// as it has pairs of vectors otherwise
-// (256 x 4096: 3.1 against 3.2; 2048 x 4096: 14.2 against 17.0; four a thread: 15.7).  Four where two are not enough for 512 threads.
+// 8192 x 512 takes 7.9 against 8.0, so those go by blocks).  Else a block of as many threads as the row has vectors while those are few for
+// the GPU (128 x 4096: 2.6 us against 2.7 with two vectors a thread), and as it has pairs of vectors otherwise (256 x 4096: 3.1 against
+// 3.2; 2048 x 4096: 14.2 against 17.0; four a thread: 15.7).  Four where two are not enough for the threads (1024 x 16384: 34 us; the kernel for
+// long rows 40).
 template <class T, int QT, bool VEC> void launch(cudaStream_t st, const NormArgs& a) {
     const int nv = ceil_div(a.C, 8), warps = 8;
     auto block = [&](int v) { return ceil_div(ceil_div(nv, v), 32) * 32; };
     if (nv <= 32) rms_norm_kernel<T, QT, 1, true, VEC><<<ceil_div(a.M, warps), 32 * warps, 0, st>>>(a);
     else if (nv <= 512 && (long long)a.M * nv <= 512 * sm_count()) rms_norm_kernel<T, QT, 1, false, VEC><<<a.M, block(1), 0, st>>>(a);
-    else if (nv <= 1024) rms_norm_kernel<T, QT, 2, false, VEC><<<a.M, block(2), 0, st>>>(a);
-    else if (nv <= 2048) rms_norm_kernel<T, QT, 4, false, VEC><<<a.M, block(4), 0, st>>>(a);
-    else rms_norm_long_kernel<T, QT, 512><<<a.M, 512, 0, st>>>(a, VEC);
+    else if (nv <= 2 * MOST<T, 2, false, VEC>) rms_norm_kernel<T, QT, 2, false, VEC><<<a.M, block(2), 0, st>>>(a);
+    else {
+        if constexpr (MOST<T, 2, false, VEC> < 1024) {
+            if (nv <= 2048) { rms_norm_kernel<T, QT, 4, false, VEC><<<a.M, block(4), 0, st>>>(a); return; }
+        }
+        rms_norm_long_kernel<T, QT, 512><<<a.M, 512, 0, st>>>(a, VEC);
+    }
 }
 template <class T, int QT> void launch(cudaStream_t st, const NormArgs& a, bool vec) { vec ? launch<T, QT, true>(st, a) : launch<T, QT, false>(st, a); }
 
