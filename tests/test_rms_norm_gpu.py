@@ -136,3 +136,19 @@ def test_streams_graphs_and_repeats():
 
 def test_no_rows():
     V.check(V.lib().vela_rms_norm_q8(None, abi.T_BF16, None, 64, None, 64, None, EPS, 0, 64, None, 64, None, 64, abi.T_I8, None, 64, None, 0))
+
+
+@pytest.mark.parametrize("C", [(1 << 31) - 8, (1 << 31) - 1])
+def test_the_longest_rows(C):
+    """columns up to an int's largest, where a block's stride past the last one is beyond it.  h is +-1 everywhere, so each 32-bit sum of squares is exact
+    but for the last ones' rounding, and y = +-2 / sqrt(1 + eps) to the bound of this file; codes are the row's largest, +-127."""
+    x = torch.ones(1, C, dtype=torch.bfloat16, device="cuda"); x[0, ::3] = -1
+    g = torch.full((C,), 2.0, dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros(1, C, dtype=torch.bfloat16, device="cuda"); q = torch.zeros(1, C, dtype=torch.int8, device="cuda"); scale = torch.zeros(1, 1, device="cuda")
+    V.check(call(abi.T_BF16, x, None, g, 1, C, None, y, abi.T_I8, q, scale, 0))
+    a = 2 / (1 + EPS) ** 0.5
+    assert abs(scale.item() * 127 / a - 1) <= REL
+    for i in range(0, C, 1 << 28):
+        sign = x[:, i:i + (1 << 28)].float()
+        assert (((y[:, i:i + (1 << 28)].float() * sign - a).abs() <= a * (ROUND[abi.T_BF16] + REL)).all())
+        assert (q[:, i:i + (1 << 28)].float() == 127 * sign).all()

@@ -157,6 +157,7 @@ template <class T, int QT, int V, bool WARP, bool VEC> __global__ void __launch_
 }
 
 // Rows too long for the registers: the inputs are read again for each step.  S is written last, since it may be X or R.
+// Columns are counted without a sign: a block's stride past the last one may lie beyond 2^31.
 template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREADS) rms_norm_long_kernel(const NormArgs a, bool vec) {
     __shared__ float red[2][THREADS / 32];
     constexpr float TOP = QT == VELA_T_I8 ? 127.f : 448.f;
@@ -164,7 +165,8 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
     const T* x = static_cast<const T*>(a.X) + row * a.ldx;
     const T* r = a.R ? static_cast<const T*>(a.R) + row * a.ldr : nullptr;
     const T* g = static_cast<const T*>(a.g);
-    auto get = [&](int c, int n, float (&h)[8]) {
+    const unsigned C = a.C;
+    auto get = [&](unsigned c, int n, float (&h)[8]) {
         load8(x + c, n, vec, h);
         if (r) {
             float t[8];
@@ -174,18 +176,18 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
         }
     };
     float ss = 0.f;
-    for (int c = 8 * threadIdx.x; c < a.C; c += 8 * THREADS) {
+    for (unsigned c = 8 * threadIdx.x; c < C; c += 8 * THREADS) {
         float h[8];
-        get(c, min(8, a.C - c), h);
+        get(c, min(8, int(C - c)), h);
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(h[i], h[i], ss);
     }
     const float rstd = rsqrtf(reduce<false>(ss, red[0], Sum()) / float(a.C) + a.eps);
     float top = 0.f;
     if (a.Q && a.qgroup == 0) {
-        for (int c = 8 * threadIdx.x; c < a.C; c += 8 * THREADS) {
+        for (unsigned c = 8 * threadIdx.x; c < C; c += 8 * THREADS) {
             float h[8], t[8];
-            const int n = min(8, a.C - c);
+            const int n = min(8, int(C - c));
             get(c, n, h);
             load8(g + c, n, vec, t);
 #pragma unroll
@@ -193,8 +195,9 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
         }
         top = reduce<false>(top, red[1], Max());
     }
-    for (int c0 = 0; c0 < a.C; c0 += 8 * THREADS) {
-        const int c = c0 + 8 * int(threadIdx.x), n = min(8, a.C - c);
+    for (unsigned c0 = 0; c0 < C; c0 += 8 * THREADS) {
+        const unsigned c = c0 + 8 * threadIdx.x;
+        const int n = min(8, int(C - c));                  // negative beyond the row
         float h[8], m = 0.f;
         if (n > 0) {
             float t[8];
@@ -221,7 +224,7 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
 // 3.2; 2048 x 4096: 14.2 against 17.0; four a thread: 15.7).  Four where two are not enough for the threads (1024 x 16384: 34 us; the kernel for
 // long rows 40).
 template <class T, int QT, bool VEC> void launch(cudaStream_t st, const NormArgs& a) {
-    const int nv = ceil_div(a.C, 8), warps = 8;
+    const int nv = (a.C - 1) / 8 + 1, warps = 8;
     auto block = [&](int v) { return ceil_div(ceil_div(nv, v), 32) * 32; };
     if (nv <= 32) rms_norm_kernel<T, QT, 1, true, VEC><<<ceil_div(a.M, warps), 32 * warps, 0, st>>>(a);
     else if (nv <= 512 && (long long)a.M * nv <= 512 * sm_count()) rms_norm_kernel<T, QT, 1, false, VEC><<<a.M, block(1), 0, st>>>(a);
