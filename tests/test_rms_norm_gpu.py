@@ -152,3 +152,15 @@ def test_the_longest_rows(C):
         sign = x[:, i:i + (1 << 28)].float()
         assert (((y[:, i:i + (1 << 28)].float() * sign - a).abs() <= a * (ROUND[abi.T_BF16] + REL)).all())
         assert (q[:, i:i + (1 << 28)].float() == 127 * sign).all()
+
+
+def test_the_most_rows():
+    """rows up to an int's largest, of the form with several rows a block"""
+    M = (1 << 31) - 1
+    x = torch.ones(M, 1, dtype=torch.bfloat16, device="cuda"); x[::3] = -1
+    g = torch.full((1,), 2.0, dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros(M, 1, dtype=torch.bfloat16, device="cuda")
+    V.check(call(abi.T_BF16, x, None, g, M, 1, None, y, abi.T_I8, None, None, 0))
+    a = 2 / (1 + EPS) ** 0.5
+    for i in range(0, M, 1 << 28):
+        assert (((y[i:i + (1 << 28)].float() * x[i:i + (1 << 28)].float() - a).abs() <= a * (ROUND[abi.T_BF16] + REL)).all())

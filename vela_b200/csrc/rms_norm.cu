@@ -226,7 +226,7 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
 template <class T, int QT, bool VEC> void launch(cudaStream_t st, const NormArgs& a) {
     const int nv = (a.C - 1) / 8 + 1, warps = 8;
     auto block = [&](int v) { return ceil_div(ceil_div(nv, v), 32) * 32; };
-    if (nv <= 32) rms_norm_kernel<T, QT, 1, true, VEC><<<ceil_div(a.M, warps), 32 * warps, 0, st>>>(a);
+    if (nv <= 32) rms_norm_kernel<T, QT, 1, true, VEC><<<(a.M - 1) / warps + 1, 32 * warps, 0, st>>>(a);
     else if (nv <= 512 && (long long)a.M * nv <= 512 * sm_count()) rms_norm_kernel<T, QT, 1, false, VEC><<<a.M, block(1), 0, st>>>(a);
     else if (nv <= 2 * MOST<T, 2, false, VEC>) rms_norm_kernel<T, QT, 2, false, VEC><<<a.M, block(2), 0, st>>>(a);
     else {
