@@ -241,7 +241,8 @@ typedef struct vela_moe {
 /* bytes of workspace for T tokens (0: arguments that vela_moe_w4 refuses).  Its contents need no preparation. */
 size_t vela_moe_w4_workspace(const vela_moe* L, int T);
 /* Y [T, D] = the layer's output for X [T, D] (`type` bf16 or f16), T <= 65535 (32 tokens at a time: the weights are read again for the next).  ids [T][topk] int32 and weights [T][topk] float
- * (largest first) are written where they are not NULL.  A NaN among a token's scores counts as the smallest score.
+ * (largest first) are written where they are not NULL.  An expert whose score is a NaN comes last in the choice, adds nothing to the
+ * softmax's sum, and has a NaN as its weight (renorm: so have the token's others) if it is chosen all the same.
  * workspace: 16-byte aligned; calls that may overlap need one each. */
 int vela_moe_w4(void* stream, int type, const void* X, int ldx, int T, const vela_moe* L, void* Y, int ldy,
                 int32_t* ids, float* weights, void* workspace, size_t workspace_bytes);

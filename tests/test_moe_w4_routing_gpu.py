@@ -1,0 +1,56 @@
+"""Routing of vela_moe_w4 where scores are not numbers, in both forms of the layer
+(tests/test_moe_w4_gpu.py has the bounds; a router of 32 bits or more than 8 tokens take the form with a routing kernel of its own).
+"""
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("no CUDA device", allow_module_level=True)
+
+from vela_b200 import abi  # noqa: E402
+from tests.test_moe_w4_gpu import Layer  # noqa: E402
+
+FORMS = [(3, False), (3, True), (20, False)]       # tokens, router in 32 bits: the form for few tokens, the other one twice
+
+
+def run(layer, x):
+    T = x.shape[0]
+    y = torch.empty_like(x)
+    ids = torch.full((T, layer.k), -1, dtype=torch.int32, device="cuda"); w = torch.empty(T, layer.k, device="cuda")
+    layer(x, y, ids, w)
+    torch.cuda.synchronize()
+    return y, ids, w
+
+
+@pytest.mark.parametrize("T,f32", FORMS)
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("bias", [False, True])
+def test_a_nan_score_comes_last(T, f32, score, bias):
+    """a router row of NaN: the other experts are scored, chosen and weighed as if it were not there"""
+    layer = Layer(21, 128, 32, 9, 3, abi.T_BF16, 64, score=score, bias=bias, router_f32=f32)
+    x = torch.randn(T, 128, generator=torch.Generator(device="cuda").manual_seed(T), device="cuda").bfloat16()
+    layer.router[4] = float("nan")
+    y, ids, w = run(layer, x)
+    assert (ids != 4).all()
+    layer.router[4] = 0                            # for the check: an expert that is out of the softmax's sum and of the choice
+    rel = layer.route(x.double())[1]
+    z = x.double() @ layer.router.double().t()
+    z[:, 4] = -torch.inf
+    p = torch.softmax(z, 1) if score == 0 else torch.sigmoid(z)
+    pick = p if layer.bias is None else p + layer.bias.double()
+    pick[:, 4] = -torch.inf
+    layer.route = lambda _: (p, rel, pick)
+    layer.check(x, y, ids, w)
+
+
+@pytest.mark.parametrize("T,f32", FORMS)
+@pytest.mark.parametrize("score", [0, 1])
+def test_a_nan_expert_that_has_to_be_chosen(T, f32, score):
+    """topk = E: the NaN comes last, with a NaN weight"""
+    layer = Layer(22, 64, 16, 5, 5, abi.T_BF16, 64, score=score, renorm=0, router_f32=f32)
+    x = torch.randn(T, 64, device="cuda").bfloat16()
+    layer.router[2] = float("nan")
+    _, ids, w = run(layer, x)
+    assert (ids[:, 4] == 2).all() and w[:, 4].isnan().all() and w[:, :4].isfinite().all()
+    assert all(sorted(r) == [0, 1, 2, 3, 4] for r in ids.tolist())

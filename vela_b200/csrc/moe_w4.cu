@@ -110,6 +110,9 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
+// an expert's share of the softmax's sum: none where the score is a NaN, so that one such expert does not spoil the others' probabilities
+__device__ __forceinline__ float soft_term(float z, float most) { return z != z ? 0.f : expf(z - most); }
+
 template <class X, class RW, int FOLD> __global__ void __cluster_dims__(RANKS, 1, 1) __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const MoeArgs a) {
     __shared__ float p[E_MAX], prob[E_MAX], top[K_MAX];
     __shared__ __align__(16) uint32_t key[E_MAX];
@@ -138,7 +141,7 @@ template <class X, class RW, int FOLD> __global__ void __cluster_dims__(RANKS, 1
     if (a.score == 0) {
         for (int e = lane; e < a.E; e += 32) m = fmaxf(m, p[e]);
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        for (int e = lane; e < a.E; e += 32) sum += expf(p[e] - m);
+        for (int e = lane; e < a.E; e += 32) sum += soft_term(p[e], m);
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
     for (int e = threadIdx.x; e < E4; e += ROUTE_WARPS * 32) {
@@ -221,7 +224,7 @@ template <class X, int FOLD, bool ZERO> __global__ void __cluster_dims__(few::RA
         if (a.score == 0) {
             for (int e = lane; e < a.E; e += 32) m = fmaxf(m, z[e]);
             for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            for (int e = lane; e < a.E; e += 32) sum += expf(z[e] - m);
+            for (int e = lane; e < a.E; e += 32) sum += soft_term(z[e], m);
             for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
         for (int e = lane; e < E4; e += 32) {
