@@ -1,4 +1,4 @@
-"""Routing of vela_moe_w4 where scores are not numbers, in both forms of the layer
+"""Routing of vela_moe_w4 where scores are not numbers or probabilities are equal in 32 bits, in both forms of the layer
 (tests/test_moe_w4_gpu.py has the bounds; a router of 32 bits or more than 8 tokens take the form with a routing kernel of its own).
 """
 import pytest
@@ -9,6 +9,7 @@ if not torch.cuda.is_available():
     pytest.skip("no CUDA device", allow_module_level=True)
 
 from vela_b200 import abi  # noqa: E402
+from tests.lm_util import sum_bound  # noqa: E402
 from tests.test_moe_w4_gpu import Layer  # noqa: E402
 
 FORMS = [(3, False), (3, True), (20, False)]       # tokens, router in 32 bits: the form for few tokens, the other one twice
@@ -54,3 +55,26 @@ def test_a_nan_expert_that_has_to_be_chosen(T, f32, score):
     _, ids, w = run(layer, x)
     assert (ids[:, 4] == 2).all() and w[:, 4].isnan().all() and w[:, :4].isfinite().all()
     assert all(sorted(r) == [0, 1, 2, 3, 4] for r in ids.tolist())
+
+
+@pytest.mark.parametrize("T,f32", FORMS)
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("top", [30.0, -130.0])
+def test_choice_between_probabilities_that_are_equal_in_32_bits(T, f32, score, top):
+    """Without a selection bias the order of the probabilities is that of the scores, also where they are all 1 or all 0 in 32 bits.  The scores
+    rise with the expert's number, by about 3 from one to the next."""
+    layer = Layer(24, 64, 16, 8, 3, abi.T_BF16, 64, score=score, renorm=0, router_f32=f32)
+    x = torch.randn(T, 64, generator=torch.Generator(device="cuda").manual_seed(T), device="cuda").bfloat16()
+    x[:, 0] = 1
+    layer.router *= 0.05
+    layer.router[:, 0] = (top + 3.0 * torch.arange(8, device="cuda")).to(layer.router.dtype)
+    if score == 0:                                 # one expert far above: the others' probabilities vanish
+        layer.router[3, 0] = top + 200
+    z = x.double() @ layer.router.double().t()
+    order = torch.sort(z, dim=1, descending=True, stable=True)
+    gap = (order.values[:, :-1] - order.values[:, 1:]).amin()
+    assert gap > 2 * sum_bound(64, x.double().abs() @ layer.router.double().abs().t()).amax()
+    _, ids, w = run(layer, x)
+    assert torch.equal(ids.long(), order.indices[:, :3])
+    p = torch.softmax(z, 1) if score == 0 else torch.sigmoid(z)
+    assert ((w.double() - p.gather(1, ids.long())).abs() <= 1e-3 * p.gather(1, ids.long()) + 2.0 ** -126).all()

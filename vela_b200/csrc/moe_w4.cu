@@ -110,6 +110,13 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
+// What the choice goes by: the larger key first.  Without a selection bias that is the score, whose order the probabilities have too, but not in 32 bits
+// where several are 0 (softmax: 104 below the largest score) or 1 (sigmoid: from 17 on).  A NaN comes last.
+__device__ __forceinline__ uint32_t choice_key(float prob, float score, const float* bias, int e) {
+    const float w = bias ? prob + __ldg(bias + e) : score;
+    return ordered(w != w ? -INFINITY : w);
+}
+
 // an expert's share of the softmax's sum: none where the score is a NaN, so that one such expert does not spoil the others' probabilities
 __device__ __forceinline__ float soft_term(float z, float most) { return z != z ? 0.f : expf(z - most); }
 
@@ -148,9 +155,8 @@ template <class X, class RW, int FOLD> __global__ void __cluster_dims__(RANKS, 1
         uint32_t v = 0;                                    // below every expert's
         if (e < a.E) {
             const float q = a.score == 0 ? expf(p[e] - m) / sum : 1.f / (1.f + expf(-p[e]));
-            const float w = q + (a.bias ? a.bias[e] : 0.f);
             prob[e] = q;
-            v = ordered(w != w ? -INFINITY : w);
+            v = choice_key(q, p[e], a.bias, e);
         }
         key[e] = v;
     }
@@ -230,9 +236,9 @@ template <class X, int FOLD, bool ZERO> __global__ void __cluster_dims__(few::RA
         for (int e = lane; e < E4; e += 32) {
             uint32_t v = 0;                                // below every expert's
             if (e < a.E) {
-                const float q = a.score == 0 ? expf(z[e] - m) / sum : 1.f / (1.f + expf(-z[e])), w = q + (a.bias ? __ldg(a.bias + e) : 0.f);
+                const float q = a.score == 0 ? expf(z[e] - m) / sum : 1.f / (1.f + expf(-z[e]));
                 s_p[warp][e] = q;
-                v = ordered(w != w ? -INFINITY : w);
+                v = choice_key(q, z[e], a.bias, e);
             }
             s_key[warp][e] = v;
         }
