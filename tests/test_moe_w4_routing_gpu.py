@@ -78,3 +78,14 @@ def test_choice_between_probabilities_that_are_equal_in_32_bits(T, f32, score, t
     assert torch.equal(ids.long(), order.indices[:, :3])
     p = torch.softmax(z, 1) if score == 0 else torch.sigmoid(z)
     assert ((w.double() - p.gather(1, ids.long())).abs() <= 1e-3 * p.gather(1, ids.long()) + 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("T,f32", FORMS)
+@pytest.mark.parametrize("score", [0, 1])
+def test_a_nan_comes_after_masked_experts(T, f32, score):
+    layer = Layer(25, 64, 16, 5, 5, abi.T_BF16, 64, score=score, renorm=0, bias=True, router_f32=f32)
+    x = torch.randn(T, 64, generator=torch.Generator(device="cuda").manual_seed(T), device="cuda").bfloat16()
+    layer.router[2] = float("nan"); layer.bias[3] = -torch.inf
+    _, ids, w = run(layer, x)
+    assert (ids[:, 3] == 3).all() and (ids[:, 4] == 2).all()
+    assert w[:, :4].isfinite().all() and w[:, 4].isnan().all()

@@ -111,10 +111,11 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 }
 
 // What the choice goes by: the larger key first.  Without a selection bias that is the score, whose order the probabilities have too, but not in 32 bits
-// where several are 0 (softmax: 104 below the largest score) or 1 (sigmoid: from 17 on).  A NaN comes last.
+// where several are 0 (softmax: 104 below the largest score) or 1 (sigmoid: from 17 on).  A NaN comes last, after experts
+// that a selection bias of minus infinity masks; 0 is left for places beyond the last expert.
 __device__ __forceinline__ uint32_t choice_key(float prob, float score, const float* bias, int e) {
     const float w = bias ? prob + __ldg(bias + e) : score;
-    return ordered(w != w ? -INFINITY : w);
+    return w != w ? 1u : ordered(w);
 }
 
 // an expert's share of the softmax's sum: none where the score is a NaN, so that one such expert does not spoil the others' probabilities
