@@ -226,8 +226,8 @@ int vela_gemv_w4(void* stream, int xtype, const void* X, int ldx, const float* x
                  const float* bias, const void* residual, int ldr, int ytype, void* Y, int ldy);
 
 /* A mixture-of-experts layer: p = softmax (score 0) or sigmoid (score 1) of X router^T; the topk largest p (+ select_bias,
- * used for the choice alone; without it the choice goes by the scores themselves) are chosen, ties to the lower expert; their p, divided by their sum where renorm is set, times
- * `scale`, weigh the experts' outputs down_e (silu(gate_e x) * (up_e x)).
+ * used for the choice alone; without it the choice goes by the scores themselves) are chosen, ties to the lower expert; their p, divided by their sum where renorm is set (also
+ * where all of them are below the smallest float), times `scale`, weigh the experts' outputs down_e (silu(gate_e x) * (up_e x)).
  * router [E][D] (the activations' type or f32); select_bias float [E] or NULL; E <= 1024, topk <= min(E, 32); D, I <= 2^20.
  * gate_up: E matrices [2 I, D], one after another, I a multiple of 8: rows 16 i .. 16 i + 7 are gate rows 8 i .. 8 i + 7 and
  * rows 16 i + 8 .. 16 i + 15 the up rows of the same numbers.  down: E matrices [D, I].  Both vela_w4's N, K are one

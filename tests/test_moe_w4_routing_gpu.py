@@ -1,4 +1,4 @@
-"""Routing of vela_moe_w4 where scores are not numbers or probabilities are equal in 32 bits, in both forms of the layer
+"""Routing of vela_moe_w4 where scores are not numbers, or probabilities equal or vanish in 32 bits, in both forms of the layer
 (tests/test_moe_w4_gpu.py has the bounds; a router of 32 bits or more than 8 tokens take the form with a routing kernel of its own).
 """
 import pytest
@@ -89,3 +89,23 @@ def test_a_nan_comes_after_masked_experts(T, f32, score):
     _, ids, w = run(layer, x)
     assert (ids[:, 3] == 3).all() and (ids[:, 4] == 2).all()
     assert w[:, :4].isfinite().all() and w[:, 4].isnan().all()
+
+
+@pytest.mark.parametrize("T,f32", FORMS)
+@pytest.mark.parametrize("score", [0, 1])
+def test_weights_of_vanishing_probabilities_sum_to_one(T, f32, score):
+    """The chosen experts' probabilities are below the smallest float; divided by their sum they are ordinary numbers.  Sigmoid: every score is
+    about -120 and less.  Softmax: the selection bias keeps the one expert out whose probability is not zero."""
+    layer = Layer(23, 64, 16, 6, 3, abi.T_BF16, 64, score=score, bias=True, router_f32=f32)
+    x = torch.randn(T, 64, generator=torch.Generator(device="cuda").manual_seed(T), device="cuda").bfloat16()
+    x[:, 0] = 1
+    layer.router *= 0.25
+    layer.router[:, 0] = (-120 - 3.0 * torch.arange(6, device="cuda")).to(layer.router.dtype)
+    layer.bias[:] = torch.tensor([3.0, 2.5, 2.0, -9.0, -9.0, -9.0], device="cuda")
+    if score == 0:
+        layer.router[5, 0] = 40.0
+    p, _, _ = layer.route(x.double())
+    assert (p[:, :3] < 2.0 ** -150).all() and (p[:, :3] > 0).all()
+    y, ids, w = run(layer, x)
+    assert w.isfinite().all() and (w.sum(1) - 1).abs().max() < 1e-5
+    layer.check(x, y, ids, w)

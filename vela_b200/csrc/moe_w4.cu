@@ -121,8 +121,25 @@ __device__ __forceinline__ uint32_t choice_key(float prob, float score, const fl
 // an expert's share of the softmax's sum: none where the score is a NaN, so that one such expert does not spoil the others' probabilities
 __device__ __forceinline__ float soft_term(float z, float most) { return z != z ? 0.f : expf(z - most); }
 
+// Weight of a token's j-th choice: its probability p[j], with `renorm` divided by the sum over the choices.  A sum below 1e-30 has probabilities in it that have
+// lost their bits or are 0; to 30 digits they are exp(score) then (sigmoid) or a multiple of it (softmax), so the scores z give the
+// quotients, taken from the largest one on.
+__device__ __forceinline__ float weight(const float* p, const float* z, int topk, int j, const MoeArgs& a) {
+    if (!a.renorm) return p[j] * a.scale;
+    float s = 0.f;
+    for (int i = 0; i < topk; ++i) s += p[i];
+    if (s < 1e-30f) {
+        float most = z[0];
+        for (int i = 1; i < topk; ++i) most = fmaxf(most, z[i]);
+        s = 0.f;
+        for (int i = 0; i < topk; ++i) s += expf(z[i] - most);
+        return expf(z[j] - most) / s * a.scale;
+    }
+    return p[j] / s * a.scale;
+}
+
 template <class X, class RW, int FOLD> __global__ void __cluster_dims__(RANKS, 1, 1) __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const MoeArgs a) {
-    __shared__ float p[E_MAX], prob[E_MAX], top[K_MAX];
+    __shared__ float p[E_MAX], prob[E_MAX], top[K_MAX], topz[K_MAX];
     __shared__ __align__(16) uint32_t key[E_MAX];
     const int E4 = (a.E + 3) & ~3;
     cg::cluster_group cluster = cg::this_cluster();
@@ -170,19 +187,15 @@ template <class X, class RW, int FOLD> __global__ void __cluster_dims__(RANKS, 1
             const uint4 k = *reinterpret_cast<const uint4*>(key + o);
             r += (k.x > v || (k.x == v && o < e)) + (k.y > v || (k.y == v && o + 1 < e)) + (k.z > v || (k.z == v && o + 2 < e)) + (k.w > v || (k.w == v && o + 3 < e));
         }
-        if (r < a.topk) { top[r] = prob[e]; a.ids[size_t(tok) * a.topk + r] = e; }
+        if (r < a.topk) { top[r] = prob[e]; topz[r] = p[e]; a.ids[size_t(tok) * a.topk + r] = e; }
     }
     __syncthreads();
-    if (int(threadIdx.x) < a.topk) {
-        float s = 0.f;
-        for (int j = 0; j < a.topk; ++j) s += top[j];
-        a.weights[size_t(tok) * a.topk + threadIdx.x] = (a.renorm ? top[threadIdx.x] / s : top[threadIdx.x]) * a.scale;
-    }
+    if (int(threadIdx.x) < a.topk) a.weights[size_t(tok) * a.topk + threadIdx.x] = weight(top, topz, a.topk, threadIdx.x, a);
 }
 
 template <class X, int FOLD, bool ZERO> __global__ void __cluster_dims__(few::RANKS, 1, 1) __launch_bounds__(few::WARPS * 32, 2) few_up_kernel(const MoeArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float s_z[few::TOKENS][few::EXPERTS], s_p[few::TOKENS][few::EXPERTS], s_top[few::PAIRS];
+    __shared__ float s_z[few::TOKENS][few::EXPERTS], s_p[few::TOKENS][few::EXPERTS], s_top[few::PAIRS], s_topz[few::PAIRS];
     __shared__ __align__(16) uint32_t s_key[few::TOKENS][few::EXPERTS];
     __shared__ int32_t s_ids[few::PAIRS];
     __shared__ float s_sum[few::WARPS][16];
@@ -256,15 +269,13 @@ template <class X, int FOLD, bool ZERO> __global__ void __cluster_dims__(few::RA
             const uint4 k = *reinterpret_cast<const uint4*>(&s_key[tok][o]);
             r += (k.x > v || (k.x == v && o < e)) + (k.y > v || (k.y == v && o + 1 < e)) + (k.z > v || (k.z == v && o + 2 < e)) + (k.w > v || (k.w == v && o + 3 < e));
         }
-        if (r < a.topk) { s_ids[tok * a.topk + r] = e; s_top[tok * a.topk + r] = s_p[tok][e]; }
+        if (r < a.topk) { s_ids[tok * a.topk + r] = e; s_top[tok * a.topk + r] = s_p[tok][e]; s_topz[tok * a.topk + r] = s_z[tok][e]; }
     }
     __syncthreads();
     if (blockIdx.x == 0 && int(threadIdx.x) < a.T * a.topk) {
-        const int tok = w4::quot(threadIdx.x, a.topk);
-        float s = 0.f;
-        for (int j = 0; j < a.topk; ++j) s += s_top[tok * a.topk + j];
+        const int at = w4::quot(threadIdx.x, a.topk) * a.topk;
         a.ids[threadIdx.x] = s_ids[threadIdx.x];
-        a.weights[threadIdx.x] = (a.renorm ? s_top[threadIdx.x] / s : s_top[threadIdx.x]) * a.scale;
+        a.weights[threadIdx.x] = weight(s_top + at, s_topz + at, a.topk, threadIdx.x - at, a);
     }
     // the hidden rows' padding
     const int wide = w4::units(a.down) * 128, P = a.T * a.topk;
