@@ -172,3 +172,16 @@ def test_no_rows():
     W = W4(1, 16, 64, 64, False, abi.T_BF16)
     c = W.c()
     V.check(V.lib().vela_gemv_w4(None, abi.T_BF16, None, 64, None, 0, 0, ctypes.byref(c), None, None, 0, abi.T_BF16, None, 16))
+
+
+@pytest.mark.parametrize("xt", [abi.T_BF16, abi.T_I8])
+def test_more_rows_than_a_grid_holds(xt):
+    """65535 times 16 rows fit a grid; a call may have more"""
+    M, N, K = 65535 * 16 + 21, 16, 32
+    gen = torch.Generator(device="cuda"); gen.manual_seed(xt)
+    W = W4(31, N, K, 32, True, abi.T_BF16)
+    x, scale, xv = make_x(gen, xt, M, K, 0, K, 0)
+    y = torch.full((M, N), float("nan"), device="cuda")
+    res = torch.randn(M, N, generator=gen, device="cuda")
+    V.check(call(xt, x, scale, 0, M, W, None, res, abi.T_F32, y))
+    check(xv, W, None, res, abi.T_F32, y)

@@ -138,7 +138,6 @@ template <int XT, int NT, int R, int BLOCKS, int FOLD, bool ZERO> __global__ voi
 template <int XT, int NT, int R, int BLOCKS, int FOLD, bool ZERO> void launch(cudaStream_t st, GemvArgs a) {
     auto* kernel = gemv_kernel<XT, NT, R, BLOCKS, FOLD, ZERO>;
     const int nrg = ceil_div(w4::row_tiles(a.W), R), nu = w4::units(a.W), mb = ceil_div(a.M, 8 * NT);
-    VELA_REQUIRE(mb <= 65535, "gemv_w4: too many rows");
     const int wave = std::max(1, sm_count() * blocks_per_sm(reinterpret_cast<const void*>(kernel), WARPS * 32, 0) / mb);
     const dim3 grid(std::min(nrg, wave), mb);
     // the split with the least time: a round costs its longest warp's units and about two more to begin and to meet
@@ -168,7 +167,22 @@ template <int XT, int NT, int R, int BLOCKS> void launch(cudaStream_t st, const 
 // 22.6 and 27.5; four column tiles in one pass would take
 // 27.5 too.  Where there is no second row tile for each SM one is faster (16x2368x4096: 4.3 against 5.1 us).  17 to 24 rows: three
 // column tiles 21.2 us at 24x8192x8192, two passes 22.3.
+constexpr int MOST_ROWS = 1 << 19;                         // of one launch: 32768 blocks of 16 along y, which takes 65535
 template <int XT> void launch(cudaStream_t st, const GemvArgs& a) {
+    if (a.M > MOST_ROWS) {
+        const size_t yb = elem_bytes(a.ytype);
+        for (int m = 0; m < a.M;) {
+            GemvArgs b = a;
+            b.M = std::min(MOST_ROWS, a.M - m);
+            b.X = static_cast<const typename w4::Act<XT>::X*>(a.X) + size_t(m) * a.ldx;
+            if (a.xscale) b.xscale = a.xscale + size_t(m) * a.nxg;
+            b.Y = static_cast<uint8_t*>(a.Y) + size_t(m) * a.ldy * yb;
+            if (a.residual) b.residual = static_cast<const uint8_t*>(a.residual) + size_t(m) * a.ldr * yb;
+            launch<XT>(st, b);
+            m += b.M;
+        }
+        return;
+    }
     if (a.M <= 8) launch<XT, 1, 1, 2>(st, a);
     else if (a.M > 16 && a.M <= 24) launch<XT, 3, 1, 1>(st, a);
     else if (w4::row_tiles(a.W) > sm_count()) launch<XT, 2, 2, 1>(st, a);
