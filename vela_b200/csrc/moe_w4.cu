@@ -28,7 +28,6 @@
 #include "w4_stream.cuh"
 #include <algorithm>
 #include <atomic>
-#include <climits>
 #include <cmath>
 #include <cooperative_groups.h>
 
@@ -43,12 +42,7 @@ constexpr int WARPS = w4::WARPS;          // of expert_kernel
 constexpr int FEW_SMEM = 96 * 1024;           // of two blocks on an SM
 constexpr size_t FEW_ROUTER = 512 * 1024;     // elements of the router that a cluster reads
 constexpr int COUNTERS = 2;               // one for each barrier
-constexpr int ROOM = 96;                  // columns times rounds whose sums expert_kernel's shared memory holds
-constexpr size_t ROOM_BYTES = w4::sum_bytes(1, ROOM);
-// Units of a row tile that a warp takes in the up phase: two share their sums' way to shared memory, but with four scales for each the
-// registers spill
-// (32 tokens, 32 experts of 4096 x 1536: groups of 64 take 118 us with two and 122 with one, groups of 32 181 and 149).
-template <int FOLD> constexpr int UP_UNITS = FOLD >= 64 ? 2 : 1;
+constexpr size_t ROOM_BYTES = w4::sum_bytes(1, w4::ROOM);
 static __device__ unsigned g_moe_err;
 
 struct MoeArgs {
@@ -449,8 +443,8 @@ template <int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS * 32, 1) 
 
     ask(a.up, share(w4::row_tiles(a.up), blockIdx.x), share(w4::row_tiles(a.up), blockIdx.x + 1));
     runs(a.up, [&](int v, size_t tile0, int r0, int r1, int c) {
-        const int nu = w4::units(a.up), room = w4::quot(ROOM, c);
-        w4::stream<w4::F, UP_UNITS<FOLD>, FOLD, ZERO, true>(a.up, tile0, r0, r1, c, a.split_up, sums, room,
+        const int nu = w4::units(a.up), room = w4::quot(w4::ROOM, c);
+        w4::stream<w4::F, w4::up_units(FOLD), FOLD, ZERO, true>(a.up, tile0, r0, r1, c, a.split_up, sums, room,
             [&](int u, uint32_t (&b)[16], w4::Pairs<FOLD>& p) {
                 auto at = [&](int col) { return size_t(a.t0 + s_tok[s_first[v] + min(col, c - 1)]) * nu + u; };     // any row where there is none: its column is not used
                 w4::load_staged<FOLD>(b, p, a.xs + at(g) * 128 + 8 * t, a.xp + at(2 * t) * (128 / FOLD), a.xp + at(2 * t + 1) * (128 / FOLD));
@@ -463,7 +457,7 @@ template <int FOLD, bool ZERO> __global__ void __launch_bounds__(WARPS * 32, 1) 
 
     const int wide = w4::row_tiles(a.down) * 16;
     runs(a.down, [&](int v, size_t tile0, int r0, int r1, int c) {
-        w4::stream<w4::H, 1, FOLD, ZERO, false>(a.down, tile0, r0, r1, c, a.split_down, sums, w4::quot(ROOM, c),
+        w4::stream<w4::H, 1, FOLD, ZERO, false>(a.down, tile0, r0, r1, c, a.split_down, sums, w4::quot(w4::ROOM, c),
             [&](int u, uint32_t (&b)[32], w4::Pairs<FOLD>& p) {
                 w4::load_floats<FOLD>(b, p, a.h + size_t(pair_of(v, min(g, c - 1))) * a.I + u * 128 + 8 * t, a.I - u * 128 - 8 * t, t);
             },
@@ -512,11 +506,9 @@ void check(const vela_moe& L, int T) {
 
 template <int FOLD, bool ZERO> void launch_experts(cudaStream_t st, MoeArgs a) {
     auto* kernel = expert_kernel<FOLD, ZERO>;
-    // as many experts as the tokens reach on average
     const int grid = sm_count();
-    const double slots = a.E * (1 - std::pow(1 - double(a.topk) / a.E, a.tn));
-    auto run = [&](const w4::Weights& W) { return std::min(w4::row_tiles(W), std::max(1, int(slots * w4::row_tiles(W) / grid))); };
-    a.split_up = w4::plan(w4::units(a.up), UP_UNITS<FOLD>, run(a.up));
+    auto run = [&](const w4::Weights& W) { return w4::run_length(w4::row_tiles(W), a.E, a.topk, a.tn, grid); };
+    a.split_up = w4::plan(w4::units(a.up), w4::up_units(FOLD), run(a.up));
     a.split_down = w4::plan(w4::units(a.down), 1, run(a.down));
     const size_t smem = ROOM_BYTES + (size_t(a.tn) * a.topk * 6 + 1 + a.E) * 4;
     constexpr size_t most = ROOM_BYTES + (size_t(T_BLOCK) * K_MAX * 6 + 1 + E_MAX) * 4;

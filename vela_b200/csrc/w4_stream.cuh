@@ -12,6 +12,7 @@
 // form; the two-term form (16 products a unit, one chain) is held up by the products' latency.
 #pragma once
 #include "w4.cuh"
+#include "w4_plan.h"
 
 namespace vela {
 namespace w4 {
@@ -154,25 +155,8 @@ __device__ __forceinline__ void multiply(float (&acc)[4], const Unit<FOLD, ZERO>
 }
 
 // ---------------------------------------------------------------- streaming row tiles past stationary activations
-constexpr int WARPS = 16;                 // of a block; one block on each SM
 constexpr int COL = 20;                   // floats from one column's 16 sums to the next: stores are free of bank conflicts
 __host__ __device__ constexpr size_t sum_bytes(int cols, int rounds) { return size_t(WARPS) * cols * COL * 4 * rounds; }
-
-// How a block splits a product: ks warps share out the units of a row tile, UW to each at a time (a chunk; several where there are
-// more), and the block takes slots = WARPS / ks
-// row tiles in a round.  The split with the least time for runs of about nrow row tiles: a chunk costs its rounds and about two more to
-// bring the activations.
-struct Split { int ks, slots, chunks; };
-inline Split plan(int nu, int uw, int nrow) {
-    Split best{1, WARPS, nu};
-    long long cost = 0;
-    for (int ks = 1; ks <= WARPS && (ks == 1 || (ks - 1) * uw < nu); ++ks) {
-        const Split s{ks, WARPS / ks, (nu + ks * uw - 1) / (ks * uw)};
-        const long long c = (long long)((nrow + s.slots - 1) / s.slots + 2) * s.chunks;
-        if (ks == 1 || c < cost) { best = s; cost = c; }
-    }
-    return best;
-}
 
 // The block's share: row tiles r0 .. r1 - 1 (at least one) of a matrix whose first row tile is number tile0, against `cols` <= 8
 // activation rows.
