@@ -266,10 +266,12 @@ template <class X, int FOLD, bool ZERO> __global__ void __cluster_dims__(few::RA
         if (r < a.topk) { s_ids[tok * a.topk + r] = e; s_top[tok * a.topk + r] = s_p[tok][e]; s_topz[tok * a.topk + r] = s_z[tok][e]; }
     }
     __syncthreads();
-    if (blockIdx.x == 0 && int(threadIdx.x) < a.T * a.topk) {
-        const int at = w4::quot(threadIdx.x, a.topk) * a.topk;
-        a.ids[threadIdx.x] = s_ids[threadIdx.x];
-        a.weights[threadIdx.x] = weight(s_top + at, s_topz + at, a.topk, threadIdx.x - at, a);
+    // The last block's last warp writes the choice: it is the one that is left without an item unless they come out even.
+    if (blockIdx.x == gridDim.x - 1 && warp == few::WARPS - 1 && lane < a.T * a.topk) {
+        static_assert(few::PAIRS <= 32, "a lane for each pair");
+        const int at = w4::quot(lane, a.topk) * a.topk;
+        a.ids[lane] = s_ids[lane];
+        a.weights[lane] = weight(s_top + at, s_topz + at, a.topk, lane - at, a);
     }
     // the hidden rows' padding
     const int wide = w4::units(a.down) * 128, P = a.T * a.topk;
