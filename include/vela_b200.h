@@ -179,7 +179,8 @@ int vela_fused_attention_stalled(void* stream, const int8_t* qhi, const int8_t* 
  * 8-bit rows, products of a few rows with 4-bit weights, and a mixture-of-experts layer on such weights.
  * Activations are 16- or 32-bit floats or 8-bit values with scales, row-major, `ld*` in elements.  Sums, norms and
  * softmax statistics are held in 32 bits.  None of the calls allocates or synchronises; each may be captured in a
- * CUDA graph.  Results do not depend on the stream, the run or what else runs (no floating-point atomics).
+ * CUDA graph.  Results do not depend on the stream, the run or what else runs (no floating-point atomics).  A row's or token's last
+ * bits may depend on how many rows or tokens share its call, since the number chooses the kernels.
  * ------------------------------------------------------------------------------ */
 #define VELA_T_BF16 0
 #define VELA_T_F16  1
@@ -218,20 +219,23 @@ int vela_w4_pack(const uint8_t* codes, const float* scales, const uint8_t* zeros
  * scale = (max(w, 0) - min(w, 0)) / 15 with zero points.  Codes are chosen for the scale as rounded. */
 int vela_w4_quantize(const float* W, int N, int K, int group, int asym, int scale_type, uint8_t* q, void* scale, uint8_t* zero);
 
-/* Y[m, n] = sum_k X[m, k] * W[n, k] + bias[n] + residual[m, n] for a few rows (any M; weights are read once for every
- * 32 rows).  X: bf16, f16, or int8 / e4m3 with xscale [M][ceil(K / xgroup)] (xgroup 64, 128) or [M] (xgroup 0).  int8 rows
+/* Y[m, n] = sum_k X[m, k] * W[n, k] + bias[n] + residual[m, n] for a few rows (any M; weights are read once for up to 8
+ * rows, for 9 to 16 and for 17 to 24, and once for every 16 of more).  X: bf16, f16, or int8 / e4m3 with xscale [M][ceil(K / xgroup)] (xgroup 64, 128) or [M] (xgroup 0).  int8 rows
  * are multiplied in integers, exactly, within each group.  bias (float [N]) and residual (Y's type) may be NULL;
  * residual may be Y itself (with the same ld).  Y: bf16, f16 or f32.  scale_type need not be xtype. */
 int vela_gemv_w4(void* stream, int xtype, const void* X, int ldx, const float* xscale, int xgroup, int M, const vela_w4* W,
                  const float* bias, const void* residual, int ldr, int ytype, void* Y, int ldy);
 
 /* A mixture-of-experts layer: p = softmax (score 0) or sigmoid (score 1) of X router^T; the topk largest p (+ select_bias,
- * used for the choice alone; without it the choice goes by the scores themselves) are chosen, ties to the lower expert; their p, divided by their sum where renorm is set (also
- * where all of them are below the smallest float), times `scale`, weigh the experts' outputs down_e (silu(gate_e x) * (up_e x)).
+ * used for the choice alone; without it the choice goes by the scores themselves) are chosen, ties to the lower expert; their p,
+ * divided by their sum where renorm is set (also where all of them are below the smallest float), times `scale`, weigh the experts'
+ * outputs down_e (silu(gate_e x) * (up_e x)).
  * router [E][D] (the activations' type or f32); select_bias float [E] or NULL; E <= 1024, topk <= min(E, 32); D, I <= 2^20.
  * gate_up: E matrices [2 I, D], one after another, I a multiple of 8: rows 16 i .. 16 i + 7 are gate rows 8 i .. 8 i + 7 and
  * rows 16 i + 8 .. 16 i + 15 the up rows of the same numbers.  down: E matrices [D, I].  Both vela_w4's N, K are one
- * expert's.  The hidden values are carried as the sum of two bf16 numbers (16 bits of precision). */
+ * expert's.  The hidden values are carried as the sum of two bf16 numbers (16 bits of precision) where a call has a few tokens and
+ * little work for each SM, else as floats that the down products take as the sum of two f16 numbers (22 bits).  An infinity among a
+ * token's activations or hidden values may make its results NaN where the formula gives an infinity. */
 typedef struct vela_moe {
     int D, I, E, topk;
     const void* router; int router_type; const float* select_bias;
@@ -240,9 +244,10 @@ typedef struct vela_moe {
 } vela_moe;
 /* bytes of workspace for T tokens (0: arguments that vela_moe_w4 refuses).  Its contents need no preparation. */
 size_t vela_moe_w4_workspace(const vela_moe* L, int T);
-/* Y [T, D] = the layer's output for X [T, D] (`type` bf16 or f16), T <= 65535 (32 tokens at a time: the weights are read again for the next).  ids [T][topk] int32 and weights [T][topk] float
- * (largest first) are written where they are not NULL.  An expert whose score is a NaN comes last in the choice, adds nothing to the
- * softmax's sum, and has a NaN as its weight (renorm: so have the token's others) if it is chosen all the same.
+/* Y [T, D] = the layer's output for X [T, D] (`type` bf16 or f16), T <= 65535 (32 tokens at a time: the weights are read again for the
+ * next).  ids [T][topk] int32 and weights [T][topk] float, in the order of the choice, are written where they are not NULL.  An
+ * expert whose score is a NaN comes last in the choice, adds nothing to the softmax's sum, and has a NaN as its weight (renorm: so
+ * have the token's others) if it is chosen all the same.
  * workspace: 16-byte aligned; calls that may overlap need one each. */
 int vela_moe_w4(void* stream, int type, const void* X, int ldx, int T, const vela_moe* L, void* Y, int ldy,
                 int32_t* ids, float* weights, void* workspace, size_t workspace_bytes);

@@ -1,5 +1,5 @@
-// Element types of the float operators: conversions between storage types and 32-bit floats, and 8-value
-// loads and stores (vector where the caller found the rows aligned, by element otherwise).
+// Element types of the float operators: conversions between storage types and 32-bit floats, and 8-value loads and stores (vector
+// where the caller found the rows aligned, by element otherwise).
 #pragma once
 #include "vela_b200.h"
 #include <cstdint>
@@ -44,9 +44,9 @@ template <class T> __device__ __forceinline__ void load_raw(Raw8<T>& x, const T*
         for (int i = 0; i < 8; ++i) if (i < n) x.e[i] = p[i];
     }
 }
-// A warp's 256 neighbouring elements (as bits E) in rows that have their type's alignment only: lane l loads and stores elements l, l + 32, ..., so that a warp's
-// 32 lie side by side; `line` (256 elements, the warp's own) brings them into the lanes' order, 8 neighbours each, and back.
-// p: the warp's first element; n: the elements that exist from there on (any number).
+// A warp's 256 neighbouring elements (as bits E) in rows that have their type's alignment only: lane l loads and stores elements l,
+// l + 32, ..., so that a warp's 32 lie side by side; `line` (256 elements, the warp's own) brings them into the lanes' order, 8
+// neighbours each, and back. p: the warp's first element; n: the elements that exist from there on (any number).
 template <class E> union Line8 { uint4 u[(sizeof(E) + 1) / 2]; uint2 h; uint32_t w[2 * sizeof(E)]; E e[8]; };
 template <class E> __device__ __forceinline__ void line_load(Line8<E>& x, const E* p, int n, int lane) {
 #pragma unroll

@@ -1,16 +1,18 @@
 // Products of a few rows with 4-bit weights: Y[m, n] = sum_k X[m, k] (code - zero) scale + bias + residual.
 //
 // The weights are read once, so with few rows the aim is to keep enough of them in flight and to spend few instructions on each.
-// The grid is one wave of 16-warp blocks that stay for the whole call.  Row group (R row tiles) i + j * grid is the j-th of block i, so
-// every SM gets about the same number; 2^ksl warps share out a group's units of 128 columns (unit u goes to warp u mod 2^ksl) and add
-// their sums in shared memory in the order of the warps.  Each warp loads one unit ahead; the many warps of an SM keep the rest in
-// flight (deeper rings in registers or shared memory cost more instructions than the latency that they hide).  Activations are read
-// through the L1 cache, which the weights pass by.
+// The grid is one wave of 16-warp blocks that stay for the whole call.  Row group (R row tiles) i + j * grid is the j-th of block
+// i, so every SM gets about the same number; 2^ksl warps share out a group's units of 128 columns (unit u goes to warp u mod 2^ksl)
+// and add their sums in shared memory in the order of the warps.  Each warp loads one unit ahead; the many warps of an SM keep the
+// rest in flight (deeper rings in registers or shared memory cost more instructions than the latency that they hide).  Activations
+// are read through the L1 cache, which the weights pass by.
 //
 // What bounds it: the issue of instructions, 140 for a unit of 16 x 128 bf16 codes with their scales (11 of them for each word of 8
-// codes), and the latency of the weights.  One row against 32768 x 8192 (139 MB with scales): 32.0 us, 4.3 TB/s, 67 % of what a copy
-// reaches (int8 28.9 us); 8192 x 8192 10.3 us, 1024 x 1024 2.5 us, of which a launch and two memory latencies are the most.  The time
-// hardly grows up to 8 rows (10.6 us); 16 rows take 13.2 us, bound by the products.
+// codes), and the latency of the weights.  One row against 32768 x 8192 (139 MB with scales): 32.0 us, 4.3 TB/s, 67 % of what a
+// copy reaches (int8 28.9 us); 8192 x 8192 10.3 us, 1024 x 1024 2.5 us, of which a launch and two memory latencies are the most.
+// The time hardly grows up to 8 rows (10.6 us).  16 rows take 13.3 us; a profile of it shows the tensor pipe 25 % and issue 32 % busy,
+// and of 11 cycles between two instructions of a warp 5 are spent on loads: the 128 registers of two column and two row tiles leave
+// room for 16 warps on an SM, too few to hide the latency of the weights and of X, which comes through L1 for every row group.
 #include "host_util.h"
 #include "w4.cuh"
 #include <algorithm>
@@ -161,12 +163,12 @@ template <int XT, int NT, int R, int BLOCKS> void launch(cudaStream_t st, const 
         else launch<XT, NT, R, BLOCKS, 128, false>(st, a);
     }
 }
-// Rows of X at a time, and one or two row tiles to a warp.  Up to 8 rows take one column tile and two blocks on an SM.  Beyond that the
-// tensor pipe bounds the kernel, and two row tiles share what is
-// read of X: 16x8192x8192 bf16 takes 13.2 us with them and 16.7 without, 32x8192x8192 (two passes over the weights, the second from L2)
-// 22.6 and 27.5; four column tiles in one pass would take
-// 27.5 too.  Where there is no second row tile for each SM one is faster (16x2368x4096: 4.3 against 5.1 us).  17 to 24 rows: three
-// column tiles 21.2 us at 24x8192x8192, two passes 22.3.
+// Rows of X at a time, and one or two row tiles to a warp.  Up to 8 rows take one column tile and two blocks on an SM.  Beyond that,
+// where there is a second row tile for each SM, two row tiles share what is read of X: 16x8192x8192 bf16 takes 13.2 us with them and
+// 16.7 without, 32x8192x8192 (two passes over the weights, the second from L2) 22.6 and 27.5; four column tiles in one pass would
+// take 27.5 too.  With few row tiles one is faster (16x2368x4096: 4.3 against 5.1 us).  The rule does not look at K, and loses up to
+// 12 % where K is short (16x6000x1024: 4.5 us with two, 4.0 with one; 16x4096x1024 3.60 and 3.36).  17 to 24 rows: three column tiles
+// 21.2 us at 24x8192x8192, two passes 22.3.
 constexpr int MOST_ROWS = 1 << 19;                         // of one launch: 32768 blocks of 16 along y, which takes 65535
 template <int XT> void launch(cudaStream_t st, const GemvArgs& a) {
     if (a.M > MOST_ROWS) {

@@ -1,16 +1,15 @@
 // The expert layer for very few tokens: every (token, expert) pair by itself, in two plain kernels.  There is next to no weight to
-// share between tokens then, and
-// latency is what counts.
-//   few_up: the four blocks of a cluster route by themselves (each forms a quarter of the scores on the tensor cores and gives them to the
-//   others through their shared memory; all of them then choose), and each takes its items of the gate and up products: an item is one row
-//   tile of one pair, ks warps share its columns.  So there is no kernel of its own for routing, nor a wait between it and the products.
-//   few_down: an item is one row tile of one token's output; its sum runs over the token's experts and their hidden columns, shared out
-//   among the block's warps.  A hidden value is the sum of two bf16 values (16 bits), which are two columns of the same product.
+// share between tokens then, and latency is what counts.
+//   few_up: the four blocks of a cluster route by themselves (each forms a quarter of the scores on the tensor cores and gives them
+//   to the others through their shared memory; all of them then choose), and each takes its items of the gate and up products: an
+//   item is one row tile of one pair, ks warps share its columns.  So there is no kernel of its own for routing, nor a wait between
+//   it and the products.
+//   few_down: an item is one row tile of one token's output; its sum runs over the token's experts and their hidden columns, shared
+//   out among the block's warps.  A hidden value is the sum of two bf16 values (16 bits), which are two columns of the same product.
 //
-// One token, 8 of 64 experts of 2048 x 1024, bf16: 16.1 us a layer, 26 MB; 2 of 16 experts of 1024 x 512: 8.2 us.  Scoring and choosing
-// take about 5 us
-// of the first kernel, the rest is latency: the first fetch of weights waits for the choice, and code that runs once comes from a cold
-// instruction cache.
+// One token, 8 of 64 experts of 2048 x 1024, bf16: 16.3 us a layer, 26 MB; 2 of 16 experts of 1024 x 512: 8.2 us.  Scoring and
+// choosing take about 5 us of the first kernel, the rest is latency: the first fetch of weights waits for the choice, and code that
+// runs once comes from a cold instruction cache.
 #pragma once
 #include "w4.cuh"
 
@@ -29,9 +28,9 @@ template <int FOLD> __host__ __device__ constexpr size_t up_bytes(int tokens, in
     return stage_bytes<FOLD>(tokens, nu) + size_t(WARPS) * score_tiles(E) * 16 * PART * 4;
 }
 
-// Scores of up to 8 tokens: this warp's share of the columns, 32 at a time, for the tiles of 16 experts rank, rank + RANKS, ...; part[e
-// * PART + token] with e counted
-// within those tiles.  X: bf16 or f16, the router's type too; D % 8 == 0, rows aligned to 16 bytes.
+// Scores of up to 8 tokens: this warp's share of the columns, 32 at a time, for the tiles of 16 experts rank, rank + RANKS, ...;
+// part[e * PART + token] with e counted within those tiles.  X: bf16 or f16, the router's type too; D % 8 == 0, rows aligned to 16
+// bytes.
 template <class X> __device__ __forceinline__ void part_scores(const X* x, int ldx, int tn, const X* router, int E, int D, float* part, int rank, int warp, int lane) {
     const int g = lane >> 2, t = lane & 3;
     const X* row = x + size_t(min(g, tn - 1)) * ldx;
@@ -55,8 +54,8 @@ template <class X> __device__ __forceinline__ void part_scores(const X* x, int l
     }
 }
 
-// Adds a unit of one row tile to acc (rows g and g + 8): one activation row, staged in shared memory (w4_stream.cuh: stage_unit).  x:
-// column 8 t of the unit.
+// Adds a unit of one row tile to acc (rows g and g + 8): one activation row, staged in shared memory (w4_stream.cuh: stage_unit).
+// x: column 8 t of the unit.
 template <int FOLD, bool ZERO>
 __device__ __forceinline__ void one_staged(float (&acc)[2], const w4::Unit<FOLD, ZERO>& W, const __half* x, const float2* pair, bool f16) {
     constexpr int HALVES = FOLD / 32;

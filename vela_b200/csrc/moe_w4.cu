@@ -1,27 +1,22 @@
-// A mixture-of-experts layer for a few tokens on 4-bit weights, in two kernels, of two forms.  What bounds the layer is the reading of
-// the chosen experts' weights; with one or
-// two tokens it is latency.
+// A mixture-of-experts layer for a few tokens on 4-bit weights, in two kernels, of two forms.  What bounds the layer is the reading
+// of the chosen experts' weights; with one or two tokens it is latency.
 //
-// Very few tokens (moe_few.cuh): few_up_kernel routes and does the gate and up products, few_down_kernel the down products and their
-// weighed sums.
+// Very few tokens (moe_few.cuh): few_up_kernel routes and does the gate and up products, few_down_kernel the down products and
+// their weighed sums.
 //
-// Else: route_kernel, a cluster of 8 blocks for each token, scores the experts (a warp for each), chooses, and stages the token's row
-// for the products (w4_stream.cuh); it also clears
-// the other kernel's counters.  expert_kernel, one block on each SM (a cooperative launch), does all chosen experts' gate and up
-// products, then their down products, then the weighed
-// sums, with a barrier over the whole grid in between.  An item is one row tile of one expert, for all tokens that chose it (columns of
-// one product, so weights are read once
-// for every 8 of them); a block takes a run of neighbouring items, so an expert's activations stay in its registers.  A barrier costs
-// about 1.5 us, over which the next
-// weights are already on their way to the L2 cache.
+// Else: route_kernel, a cluster of 8 blocks for each token, scores the experts (a warp for each), chooses, and stages the token's
+// row for the products (w4_stream.cuh); it also clears the other kernel's counters.  expert_kernel, one block on each SM (a
+// cooperative launch), does all chosen experts' gate and up products, then their down products, then the weighed sums, with a
+// barrier over the whole grid in between.  An item is one row tile of one expert, for all tokens that chose it (columns of one
+// product, so weights are read once for every 8 of them); a block takes a run of neighbouring items, so an expert's activations
+// stay in its registers.  A barrier costs about 1.5 us, over which the next weights are already on their way to the L2 cache.
 //   Up: a row tile is 8 gate rows and their 8 up rows, so one thread sums both parts of a hidden value, which is kept as a float.
-//   Down: the result of each token and expert by itself, as floats; then each output is summed over the token's experts in the order of
-//   their places.
-// 32 tokens, 4 of 32 experts of 4096 x 1536, bf16: 101 us for 308 MB, 47 % of what a copy reaches.  Routing and the gap to the next
-// kernel take 10 us; blocks end
-// up to 12 us apart in each phase (their shares are equal, their bandwidth is not; handing out the last items as blocks get free costs
-// more,
-// since every run begins anew), and the down phase is bound by its products' latency.
+//   Down: the result of each token and expert by itself, as floats; then each output is summed over the token's experts in the
+//   order of their places.
+// 32 tokens, 4 of 32 experts of 4096 x 1536, bf16: 101 to 103 us for 308 MB, 46 % of what a copy reaches.  Routing and the gap to
+// the next kernel take 10 us; blocks end up to 12 us apart in each phase (their shares are equal, their bandwidth is not; handing out
+// the last items as blocks get free costs more, since every run begins anew), and the down phase has a chain of 16 dependent products
+// for each unit.
 #include "host_util.h"
 #include "tc.cuh"
 #include "moe_few.cuh"
@@ -104,20 +99,21 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// What the choice goes by: the larger key first.  Without a selection bias that is the score, whose order the probabilities have too, but not in 32 bits
-// where several are 0 (softmax: 104 below the largest score) or 1 (sigmoid: from 17 on).  A NaN comes last, after experts
-// that a selection bias of minus infinity masks; 0 is left for places beyond the last expert.
+// What the choice goes by: the larger key first.  Without a selection bias that is the score, whose order the probabilities have
+// too, but not in 32 bits where several are 0 (softmax: 104 below the largest score) or 1 (sigmoid: from 17 on).  A NaN comes last,
+// after experts that a selection bias of minus infinity masks; 0 is left for places beyond the last expert.
 __device__ __forceinline__ uint32_t choice_key(float prob, float score, const float* bias, int e) {
     const float w = bias ? prob + __ldg(bias + e) : score;
     return w != w ? 1u : ordered(w);
 }
 
-// an expert's share of the softmax's sum: none where the score is a NaN, so that one such expert does not spoil the others' probabilities
+// an expert's share of the softmax's sum: none where the score is a NaN, so that one such expert does not spoil the others'
+// probabilities
 __device__ __forceinline__ float soft_term(float z, float most) { return z != z ? 0.f : expf(z - most); }
 
-// Weight of a token's j-th choice: its probability p[j], with `renorm` divided by the sum over the choices.  A sum below 1e-30 has probabilities in it that have
-// lost their bits or are 0; to 30 digits they are exp(score) then (sigmoid) or a multiple of it (softmax), so the scores z give the
-// quotients, taken from the largest one on.
+// Weight of a token's j-th choice: its probability p[j], with `renorm` divided by the sum over the choices.  A sum below 1e-30 has
+// probabilities in it that have lost their bits or are 0; to 30 digits they are exp(score) then (sigmoid) or a multiple of it
+// (softmax), so the scores z give the quotients, taken from the largest one on.
 __device__ __forceinline__ float weight(const float* p, const float* z, int topk, int j, const MoeArgs& a) {
     if (!a.renorm) return p[j] * a.scale;
     float s = 0.f;
@@ -148,7 +144,7 @@ template <class X, class RW, int FOLD> __global__ void __cluster_dims__(RANKS, 1
     }
     cluster.sync();
     if (rank != 0) {
-        // the others: the staged row, the hidden rows' padding, the counters
+        // the others: the staged row and the counters
         const int i = gw - ROUTE_WARPS, n = (RANKS - 1) * ROUTE_WARPS, nu = w4::units(a.up);
         for (int u = i; u < nu; u += n)
             w4::stage_unit<X, FOLD>(x + u * 128 + 4 * lane, a.D - u * 128 - 4 * lane, a.xs + (size_t(tok) * nu + u) * 128, a.xp + (size_t(tok) * nu + u) * (128 / FOLD), lane);
@@ -323,8 +319,8 @@ template <int FOLD, bool ZERO, int WARPS> __global__ void __launch_bounds__(WARP
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rt = w4::row_tiles(a.down), nu = w4::units(a.down), items = a.T * rt, n = a.topk * nu, wide = nu * 128;
     const w4::Consts k = w4::consts<__nv_bfloat16>();
-    // few_up_kernel has ended and its results are visible; they were written while this kernel was already there, so all are read by
-    // plain loads
+    // few_up_kernel has ended and its results are visible; they were written while this kernel was already there, so all are read
+    // by plain loads
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // the two terms of a hidden value are columns 0 and 1 of the product (and 2 to 7 again, which are not used)
     const __nv_bfloat16* h = (g & 1 ? a.lo : a.hi) + 8 * t;
@@ -524,17 +520,15 @@ template <class X, int FOLD, bool ZERO> void launch_few(cudaStream_t st, MoeArgs
     const size_t smem = few::up_bytes<FOLD>(a.T, w4::units(a.up), a.E);
     static std::atomic<int> ready[64];
     once_per_device(ready, [&] { VELA_CUDA(cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM)); });
-    // no more clusters than run at a time (71 of 2 x 148 blocks; the others would wait for a whole kernel); all of a block's items in
-    // one round if there are warps for it, since a
-    // round costs a memory latency
+    // no more clusters than run at a time (71 of 2 x 148 blocks; the others would wait for a whole kernel); all of a block's items
+    // in one round if there are warps for it, since a round costs a memory latency
     const int items = a.T * a.topk * w4::row_tiles(a.up);
     const int grid = std::min(ceil_div(items, few::RANKS), clusters_per_device(reinterpret_cast<const void*>(up), few::RANKS, few::WARPS * 32, smem)) * few::RANKS;
     const int ks = std::max(1, std::min(w4::units(a.up), few::WARPS / ceil_div(items, grid)));
     a.split_up = w4::Split{ks, few::WARPS / ks, 1};
     up<<<grid, few::WARPS * 32, smem, st>>>(a);
-    // 32 warps on a row tile where there is one for an SM at most, so that each has half as many units one after another (E = 64, D =
-    // 2048: 18.6 -> 16.1 us a layer), else two blocks of 16
-    // (D = 4096, where 32 took 22.3 us against 20.8)
+    // 32 warps on a row tile where there is one for an SM at most, so that each has half as many units one after another (E = 64,
+    // D = 2048: 18.6 -> 16.1 us a layer when it was chosen), else two blocks of 16 (D = 4096, where 32 took 22.3 us against 20.8)
     const int rows = a.T * w4::row_tiles(a.down), sms = sm_count();
     const bool wide = rows <= sms && a.topk * w4::units(a.down) > 16;
     // brought up while the first is still running; it waits for it before it reads anything
@@ -550,9 +544,8 @@ template <int FOLD> void launch_few(cudaStream_t st, const MoeArgs& a) {
     else a.up.zero ? launch_few<__half, FOLD, true>(st, a) : launch_few<__half, FOLD, false>(st, a);
 }
 // Which form.  Measured over 1 to 8 tokens, widths 512 to 4096, 8 to 128 experts of 256 to 2048, by the gate and up units of 128
-// columns for each SM and one and a half times the
-// units of the tokens' rows, which every block stages: the few-token form takes 7 to 24 us against 16 to 32 of the other up to 330, and
-// 39 against 38 at 540, 36 against 28 at 490.
+// columns for each SM and one and a half times the units of the tokens' rows, which every block stages: the few-token form takes 7
+// to 24 us against 16 to 32 of the other up to 330, and 39 against 38 at 540, 36 against 28 at 490.
 template <int FOLD> bool is_few(const MoeArgs& a, int router_type) {
     const double units = double(a.T) * a.topk * w4::row_tiles(a.up) * w4::units(a.up) / sm_count() + 1.5 * a.T * w4::units(a.up);
     return units <= 430 && a.T <= few::TOKENS && a.E <= few::EXPERTS && a.T * a.topk <= few::PAIRS && router_type == a.ytype && a.vecx && a.vecr &&

@@ -1,9 +1,9 @@
 // Residual addition, root-mean-square norm and 8-bit quantisation of rows in one pass:
 //   h = X + R,  S = h,  y = h * rsqrt(mean(h^2) + eps) * g,  Y = y,  Q = y / scale.
-// h stays in 32-bit registers between the two reductions (the mean square, and the largest |y| of a row or group
-// of columns), so each input is read once and each output written once: memory bounds it, from some thousand rows on, and for few rows
-// the launch and one memory latency.  8192 x 4096 bf16 with a residual, S and 8-bit groups: 39.6 us, 5.96 TB/s, 92 % of what a copy
-// reaches; 1003 x 5000 f16 8.9 us (61 %); 77 x 1024 f32 2.3 us.
+// h stays in 32-bit registers between the two reductions (the mean square, and the largest |y| of a row or group of columns), so each
+// input is read once and each output written once: memory bounds it, from some thousand rows on, and for few rows the launch and one
+// memory latency.  8192 x 4096 bf16 with a residual, S and 8-bit groups: 39.5 us, 5.97 TB/s, 93 % of what a copy reaches; 1003 x 5000
+// f16 8.9 us (61 %); 77 x 1024 f32 2.3 us.
 #include "elem.cuh"
 #include "host_util.h"
 #include "vela_b200.h"
@@ -53,12 +53,14 @@ __device__ __forceinline__ void store_q8(uint8_t* p, int n, bool vec, const Byte
         for (int i = 0; i < 8; ++i) if (i < n) p[i] = o.b[i];
 }
 
-// A block, or with WARP a warp, for each row; thread i holds values 8 (i + j n) .. + 7, j < V, in registers, n the row's threads.  All three
-// inputs are fetched before the first reduction.  The group of 64 or 128 columns is 8 or 16 neighbouring lanes.  VEC: rows are whole and
-// aligned vectors; others are loaded and stored with a warp's 32 elements side by side and brought into the lanes' order in shared memory
-// (elem.cuh): 8192 x 4095 bf16 takes 80 us so, 131 with each lane on its own 8 elements (and 126 by aligned blocks shifted into place).
-// threads; without alignment a block of 1024 is better than four vectors a thread, whose 107 registers leave room for one block
-// (2000 x 10241 f16: 79 us against 103), with it the smaller bound is (8192 x 4096 bf16: 39.5 against 40.5)
+// A block, or with WARP a warp, for each row; thread i holds values 8 (i + j n) .. + 7, j < V, in registers, n the row's threads.
+// All three inputs are fetched before the first reduction.  The group of 64 or 128 columns is 8 or 16 neighbouring lanes.  VEC:
+// rows are whole and aligned vectors; others are loaded and stored with a warp's 32 elements side by side and brought into the
+// lanes' order in shared memory (elem.cuh): 8192 x 4095 bf16 takes 80 us so, 131 with each lane on its own 8 elements (and 126 by
+// aligned blocks shifted into place).
+//
+// MOST: the threads of a block.  Without alignment a block of 1024 is better than four vectors a thread, whose 107 registers leave
+// room for one block (2000 x 10241 f16: 79 us against 103); with it the smaller bound is (8192 x 4096 bf16: 39.5 against 40.5).
 template <class T, int V, bool WARP, bool VEC> constexpr int MOST = WARP ? 256 : V == 2 && sizeof(T) == 2 && !VEC ? 1024 : 512;
 template <class T, int QT, int V, bool WARP, bool VEC> __global__ void __launch_bounds__(MOST<T, V, WARP, VEC>) rms_norm_kernel(const NormArgs a) {
     __shared__ float red[2][MOST<T, V, WARP, VEC> / 32];
@@ -156,8 +158,8 @@ template <class T, int QT, int V, bool WARP, bool VEC> __global__ void __launch_
     }
 }
 
-// Rows too long for the registers: the inputs are read again for each step.  S is written last, since it may be X or R.
-// Columns are counted without a sign: a block's stride past the last one may lie beyond 2^31.
+// Rows too long for the registers: the inputs are read again for each step.  S is written last, since it may be X or R.  Columns are
+// counted without a sign: a block's stride past the last one may lie beyond 2^31.
 template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREADS) rms_norm_long_kernel(const NormArgs a, bool vec) {
     __shared__ float red[2][THREADS / 32];
     constexpr float TOP = QT == VELA_T_I8 ? 127.f : 448.f;
@@ -218,11 +220,11 @@ template <class T, int QT, int THREADS> __global__ void __launch_bounds__(THREAD
     }
 }
 
-// A warp a row where it has one vector for each lane (8192 x 256 bf16: 3.7 us against 6.1 with a block a row; with two for each lane
-// 8192 x 512 takes 7.9 against 8.0, so those go by blocks).  Else a block of as many threads as the row has vectors while those are few for
-// the GPU (128 x 4096: 2.6 us against 2.7 with two vectors a thread), and as it has pairs of vectors otherwise (256 x 4096: 3.1 against
-// 3.2; 2048 x 4096: 14.2 against 17.0; four a thread: 15.7).  Four where two are not enough for the threads (1024 x 16384: 34 us; the kernel for
-// long rows 40).
+// A warp a row where it has one vector for each lane (8192 x 256 bf16: 3.7 us against 6.1 with a block a row; with two for each
+// lane 8192 x 512 takes 7.9 against 8.0, so those go by blocks).  Else a block of as many threads as the row has vectors while
+// those are few for the GPU (128 x 4096: 2.6 us against 2.7 with two vectors a thread), and as it has pairs of vectors otherwise
+// (256 x 4096: 3.1 against 3.2; 2048 x 4096: 14.2 against 17.0; four a thread: 15.7).  Four where two are not enough for the
+// threads (1024 x 16384: 34 us; the kernel for long rows 40).
 template <class T, int QT, bool VEC> void launch(cudaStream_t st, const NormArgs& a) {
     const int nv = (a.C - 1) / 8 + 1, warps = 8;
     auto block = [&](int v) { return ceil_div(ceil_div(nv, v), 32) * 32; };

@@ -1,16 +1,15 @@
-// 4-bit weight tiles on the tensor cores: the 16 x 64 tile of vela_w4 (512 bytes, 16 per lane) against up to 8 NT
-// activation rows.
+// 4-bit weight tiles on the tensor cores: the 16 x 64 tile of vela_w4 (512 bytes, 16 per lane) against up to 8 NT activation rows.
 //
-// Lane 4 g + t of a warp holds, in word j (j < 4) of its 16 bytes, rows g and g + 8 at the four columns
-// k = 32 (j / 2) + 8 t + 4 (j % 2) + {0, 1, 2, 3}.  A product over k does not mind in which order k runs, so those columns stand in
-// the places that the instruction numbers 2t, 2t + 1, 2t + 8, 2t + 9 (16-bit operands) or 4t .. 4t + 3 (8-bit ones), for
-// the weights and the activations alike.  Of a word's nibbles 0..7, (0, 4) and (2, 6) are row g's column pairs (0, 1) and (2, 3),
-// (1, 5) and (3, 7) row g + 8's.
+// Lane 4 g + t of a warp holds, in word j (j < 4) of its 16 bytes, rows g and g + 8 at the four columns k = 32 (j / 2) + 8 t + 4 (j
+// % 2) + {0, 1, 2, 3}.  A product over k does not mind in which order k runs, so those columns stand in the places that the
+// instruction numbers 2t, 2t + 1, 2t + 8, 2t + 9 (16-bit operands) or 4t .. 4t + 3 (8-bit ones), for the weights and the
+// activations alike.  Of a word's nibbles 0..7, (0, 4) and (2, 6) are row g's column pairs (0, 1) and (2, 3), (1, 5) and (3, 7) row
+// g + 8's.
 //
-// 16-bit operands: 0x4300 | n is the bf16 number 128 + n and 0x6400 | n the f16 number 1024 + n (0x5400 | n << 4 the number 64 + n, which
-// saves a shift), from which 128 + zero (1024 + zero, 64 + zero) is taken exactly: the operand is the integer code - zero, and nothing is
-// rounded before the 32-bit accumulation.  8-bit operands: a mask leaves the unsigned byte code (row g) or 16 * code (row g + 8), and zero
-// times the sum of the activations, from one more product by ones, is taken off the 32-bit integer sum.
+// 16-bit operands: 0x4300 | n is the bf16 number 128 + n and 0x6400 | n the f16 number 1024 + n (0x5400 | n << 4 the number 64 + n,
+// which saves a shift), from which 128 + zero (1024 + zero, 64 + zero) is taken exactly: the operand is the integer code - zero,
+// and nothing is rounded before the 32-bit accumulation.  8-bit operands: a mask leaves the unsigned byte code (row g) or 16 * code
+// (row g + 8), and zero times the sum of the activations, from one more product by ones, is taken off the 32-bit integer sum.
 #pragma once
 #include "elem.cuh"
 #include "vela_b200.h"
@@ -77,8 +76,8 @@ template <class M> __device__ __forceinline__ Consts consts() {
 }
 template <> __device__ __forceinline__ Consts consts<int8_t>() { return Consts{}; }
 
-// a / b for a >= 0, b > 0: the quotient of floats is off by a few at most, which the loops put right (a division of integers takes many
-// times as long)
+// a / b for a >= 0, b > 0: the quotient of floats is off by a few at most, which the loops put right (a division of integers takes
+// many times as long)
 __device__ __forceinline__ int quot(int a, int b) {
     int q = int(__fdividef(float(a), float(b))), r = a - q * b;
     while (r < 0) { --q; r += b; }
@@ -99,9 +98,8 @@ __device__ __forceinline__ uint4 load_tile(const uint4* p) {
     return v;
 }
 
-// A unit is two neighbouring tiles (128 columns) of one row tile: what a warp loads at once.  FOLD (32, 64 or 128) is the
-// number of columns between scalings, the smaller of the weights' and the activations' group; a unit has one scale (and zero) for each
-// fold.
+// A unit is two neighbouring tiles (128 columns) of one row tile: what a warp loads at once.  FOLD (32, 64 or 128) is the number of
+// columns between scalings, the smaller of the weights' and the activations' group; a unit has one scale (and zero) for each fold.
 template <int FOLD, bool ZERO> struct Unit {
     uint4 w[2];
     uint32_t s[128 / FOLD];
@@ -134,8 +132,8 @@ template <int FOLD, bool ZERO> __device__ __forceinline__ void load_unit(Unit<FO
         if constexpr (ZERO) o.z[f] = __ldg(p.z + grp * 8);
     }
 }
-// The last unit (number u) may lack its second tile or its last groups: the last tile and group are read again in their
-// place, and meet activations of zero.
+// The last unit (number u) may lack its second tile or its last groups: the last tile and group are read again in their place, and
+// meet activations of zero.
 template <int FOLD, bool ZERO> __device__ __forceinline__ void load_last(Unit<FOLD, ZERO>& o, const RowPtr& p, const Weights& W, int u) {
     o.w[0] = load_tile(p.q);
     o.w[1] = load_tile(p.q + (2 * u + 1 < W.kt ? 32 : 0));
@@ -155,9 +153,8 @@ template <> struct Act<VELA_T_F16> { typedef __half X; typedef __half M; static 
 template <> struct Act<VELA_T_E4M3> { typedef uint8_t X; typedef __half M; static constexpr bool scaled = true, integer = false; static constexpr int REGS = 4; };
 template <> struct Act<VELA_T_I8> { typedef uint8_t X; typedef int8_t M; static constexpr bool scaled = true, integer = true; static constexpr int REGS = 2; };
 
-// A lane's 8 activations p[0 .. 8) of a 32-column part as operands.  Not WHOLE: n of them exist (may be negative), zeros stand for the
-// others,
-// and p has its type's alignment only.  CONSTANT: nobody writes them while the kernel is there.
+// A lane's 8 activations p[0 .. 8) of a 32-column part as operands.  Not WHOLE: n of them exist (may be negative), zeros stand for
+// the others, and p has its type's alignment only.  CONSTANT: nobody writes them while the kernel is there.
 template <int XT, bool WHOLE, bool CONSTANT = true> __device__ __forceinline__ void load_x8(uint32_t (&b)[Act<XT>::REGS], const typename Act<XT>::X* p, int n) {
     static_assert(CONSTANT || sizeof(typename Act<XT>::X) == 2, "8-bit rows are always read as constants");
     if constexpr (sizeof(typename Act<XT>::X) == 2) {
@@ -193,12 +190,10 @@ template <int XT, bool WHOLE, bool CONSTANT = true> __device__ __forceinline__ v
     }
 }
 
-// Adds one unit of R row tiles to acc: c0, c1 = row g and activation rows 2t, 2t + 1; c2, c3 = row g + 8.  x[n]: this lane's place (row
-// g of column
-// tile n, column 8 t of the unit; any row where there is none: its column of the product is not used); WHOLE: all 128 columns exist and
-// x is aligned
-// to 8 of them, else left columns exist from x on; sx(f, n): the scales of activation rows 2t, 2t + 1 of column tile n in fold f (8-bit
-// forms).
+// Adds one unit of R row tiles to acc: c0, c1 = row g and activation rows 2t, 2t + 1; c2, c3 = row g + 8.  x[n]: this lane's place
+// (row g of column tile n, column 8 t of the unit; any row where there is none: its column of the product is not used); WHOLE: all
+// 128 columns exist and x is aligned to 8 of them, else left columns exist from x on; sx(f, n): the scales of activation rows 2t,
+// 2t + 1 of column tile n in fold f (8-bit forms).
 template <int XT, bool WHOLE, int NT, int R, bool CONSTANT = true, int FOLD, bool ZERO, class SX>
 __device__ __forceinline__ void unit(float (&acc)[R][NT][4], const Unit<FOLD, ZERO> (&W)[R], const typename Act<XT>::X* const (&x)[NT], int left, bool f16,
                                      const Consts& k, SX sx) {

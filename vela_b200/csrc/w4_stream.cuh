@@ -1,15 +1,14 @@
 // Streaming row tiles of 4-bit weights past stationary activations, for products in which a block has many row tiles and the same
 // few activation rows.
 //
-// A warp keeps the activations of UW units (128 columns each) in registers and streams row tiles past them, so they are read once for many
-// row tiles.  They are f16 (exactly: f16 as it is, bf16 and float with a power of two for each row and 128 columns; floats as the sum
-// of two).  The bits of a nibble
-// at the bottom of a 16-bit half are, as they stand, the (subnormal) f16 number code * 2^-24, four bits up code * 2^-20, both exact and
-// taken by
-// the tensor cores at full rate: a word of 8 codes takes one shift and four masks and no conversion (w4.cuh's direct forms: 9 to 11).
-// Zero times the activations' sum is taken off the sum of products.  A unit costs 3 loads, 40 instructions of decoding, 8 products and
-// 12 to 16 for its scales.  While a block's loop runs it takes 41 bytes of weights a nanosecond (6.1 TB/s over all SMs) in the one-term
-// form; the two-term form (16 products a unit, one chain) is held up by the products' latency.
+// A warp keeps the activations of UW units (128 columns each) in registers and streams row tiles past them, so they are read once
+// for many row tiles.  They are f16 (exactly: f16 as it is, bf16 and float with a power of two for each row and 128 columns; floats
+// as the sum of two).  The bits of a nibble at the bottom of a 16-bit half are, as they stand, the (subnormal) f16 number code *
+// 2^-24, four bits up code * 2^-20, both exact and taken by the tensor cores at full rate: a word of 8 codes takes one shift and
+// four masks and no conversion (w4.cuh's direct forms: 9 to 11).  Zero times the activations' sum is taken off the sum of products.
+// A unit costs 3 loads, 40 instructions of decoding, 8 products and 12 to 16 for its scales.  While a block's loop runs it takes 41
+// bytes of weights a nanosecond (6.1 TB/s over all SMs) in the one-term form; the two-term form has 16 products a unit in one
+// chain and takes about half of that.
 #pragma once
 #include "w4.cuh"
 #include "w4_plan.h"
@@ -26,12 +25,12 @@ __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
 // F: f16 values.  H: the sum of two f16 values (22 bits).  regs: a lane's registers for one unit and 8 rows.
 enum Kind { F, H };
 template <Kind KIND> __host__ __device__ constexpr int regs() { return KIND == F ? 16 : 32; }
-// For each fold and the lane's two columns of the product (rows 2t and 2t + 1 of the activations): the factor that the operands have
-// lost, and their sum.
+// For each fold and the lane's two columns of the product (rows 2t and 2t + 1 of the activations): the factor that the operands
+// have lost, and their sum.
 template <int FOLD> struct Pairs { float2 v[128 / FOLD][2]; };
 
-// Fills in the pairs of H: the sums come out of a product by ones where they are needed, the factor (known to the four lanes of row g)
-// by a shuffle.
+// Fills in the pairs of H: the sums come out of a product by ones where they are needed, the factor (known to the four lanes of row
+// g) by a shuffle.
 template <int FOLD> __device__ __forceinline__ void make_pairs(Pairs<FOLD>& p, const uint32_t (&b)[32], int t, float lost) {
     constexpr int HALVES = FOLD / 32;
     const float e = __shfl_sync(0xffffffffu, lost, 8 * t), o = __shfl_sync(0xffffffffu, lost, 8 * t + 4);
@@ -51,8 +50,8 @@ template <int FOLD> __device__ __forceinline__ void make_pairs(Pairs<FOLD>& p, c
 }
 
 // The power of two that brings a row's 128 values (top: the bits of the largest magnitude among a lane's 32) into f16's range, the
-// largest to [2^14, 2^15), and its inverse.  bf16's 8 bits
-// then fit exactly down to 2^-31 of the largest, and what is smaller is rounded to 2^-39 of it, below a 32-bit sum's own rounding.
+// largest to [2^14, 2^15), and its inverse.  bf16's 8 bits then fit exactly down to 2^-31 of the largest, and what is smaller is
+// rounded to 2^-39 of it, below a 32-bit sum's own rounding.
 __device__ __forceinline__ float2 row_scale(uint32_t top) {
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -65,8 +64,8 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One unit of a staged row (stage_unit): x this lane's row g from column 8 t of the unit on, e and o the unit's pairs of the rows 2t
-// and 2t + 1.
+// One unit of a staged row (stage_unit): x this lane's row g from column 8 t of the unit on, e and o the unit's pairs of the rows
+// 2t and 2t + 1.
 template <int FOLD> __device__ __forceinline__ void load_staged(uint32_t (&b)[16], Pairs<FOLD>& p, const __half* x, const float2* e, const float2* o) {
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
@@ -93,9 +92,8 @@ template <class X, int FOLD> __device__ __forceinline__ void stage_values(float 
     for (int o = 1; o < FOLD / 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane % (FOLD / 4) == 0) pair[lane / (FOLD / 4)] = make_float2(s.y, sum);
 }
-// Stages one unit of a row of X, a warp together: columns 4 lane .. 4 lane + 3 (n of them exist, from p on) to `out` (the unit's 128
-// values); the first lane of each fold writes its
-// pair {factor that the staged values have lost, their sum}.
+// Stages one unit of a row of X, a warp together: columns 4 lane .. 4 lane + 3 (n of them exist, from p on) to `out` (the unit's
+// 128 values); the first lane of each fold writes its pair {factor that the staged values have lost, their sum}.
 template <class X, int FOLD> __device__ __forceinline__ void stage_unit(const X* p, int n, __half* out, float2* pair, int lane) {
     float v[4];
 #pragma unroll
@@ -159,10 +157,9 @@ constexpr int COL = 20;                   // floats from one column's 16 sums to
 __host__ __device__ constexpr size_t sum_bytes(int cols, int rounds) { return size_t(WARPS) * cols * COL * 4 * rounds; }
 
 // The block's share: row tiles r0 .. r1 - 1 (at least one) of a matrix whose first row tile is number tile0, against `cols` <= 8
-// activation rows.
-// Weights are loaded one round ahead.  A warp's sums go to shared memory and are added there, in the order of the warps, once for `room`
-// rounds (sum_bytes).  load(u, b, pairs): operands of unit u, by a whole warp; out(rt, col, row or half row, sums):
-// called by one thread for each row of 16, or with PAIRED for each i < 8 with the sums of rows i and i + 8.
+// activation rows.  Weights are loaded one round ahead.  A warp's sums go to shared memory and are added there, in the order of the
+// warps, once for `room` rounds (sum_bytes).  load(u, b, pairs): operands of unit u, by a whole warp; out(rt, col, row or half row,
+// sums): called by one thread for each row of 16, or with PAIRED for each i < 8 with the sums of rows i and i + 8.
 template <Kind KIND, int UW, int FOLD, bool ZERO, bool PAIRED, class LOAD, class OUT>
 __device__ __forceinline__ void stream(const Weights& W, size_t tile0, int r0, int r1, int cols, const Split& split, float* sums, int room, LOAD load, OUT out) {
     typedef Unit<FOLD, ZERO> U;
@@ -175,8 +172,7 @@ __device__ __forceinline__ void stream(const Weights& W, size_t tile0, int r0, i
     auto count = [&](int base, int n) { return sl < slots ? max(0, min(n, total - base)) : 0; };      // rounds with a row tile for this warp
 
     // Where the next round to be loaded lies, for a chunk's UW units.  Units beyond the last are the last one again, and so are the
-    // second tile and the groups that the
-    // last unit may lack: they meet activations of zero.
+    // second tile and the groups that the last unit may lack: they meet activations of zero.
     const uint4* fq = nullptr;
     const uint32_t* fs = nullptr;
     const uint16_t* fz = nullptr;
